@@ -274,6 +274,16 @@ from bluefog_amd.optimizers import (  # noqa: E402
 )
 
 # ---------------------------------------------------------------------------
+# transformer training operators
+# ---------------------------------------------------------------------------
+
+from bluefog_amd.ops.transformer import (  # noqa: E402
+    counter_dropout,
+    layer_norm,
+    packed_attention,
+)
+
+# ---------------------------------------------------------------------------
 # utilities & topology library
 # ---------------------------------------------------------------------------
 

@@ -244,6 +244,9 @@ void ln_add_bwd(at::Tensor dx, at::Tensor x, at::Tensor r, at::Tensor dy,
 
 }  // namespace
 
+// transformer_ops.cpp: packed attention, layer norm, counter-based dropout
+void bf_register_transformer_ops(py::module& m);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "bluefog_amd native CDNA4 kernels (gfx950)";
   m.def("weighted_combine", &weighted_combine,
@@ -264,4 +267,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ln_bwd_scratch_rows",
         [](long nrows) { return bf_ln_bwd_scratch_rows(nrows); },
         "workgroup slots the ln_add_bwd scratch buffer must provide");
+  bf_register_transformer_ops(m);
 }

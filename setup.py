@@ -19,10 +19,16 @@ ext = CUDAExtension(
     sources=[
         "bluefog_amd/csrc/bindings.cpp",
         "bluefog_amd/csrc/bluefog_kernels.hip",
+        "bluefog_amd/csrc/transformer_ops.cpp",
+        "bluefog_amd/csrc/attention.hip",
+        "bluefog_amd/csrc/norm.hip",
     ],
     extra_compile_args={
         "cxx": ["-O3", "-std=c++17"],
-        "nvcc": ["-O3", "-std=c++17"],
+        # no packed 32-bit float instructions: some of their forms have given
+        # wrong results on gfx950, without an error and not reproducibly
+        "nvcc": ["-O3", "-std=c++17",
+                 "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"],
     },
 )
 
