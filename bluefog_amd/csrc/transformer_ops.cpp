@@ -331,7 +331,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     a.dbias = got[3].defined() ? got[3].data_ptr() : nullptr;
     Tensor partial;
     if (a.dweight || a.dbias) {
-      partial = at::empty({bf_norm_partial_floats(a.rows, a.width, code_of(x), code_of(kind))},
+      partial = at::empty({bf_norm_partial_floats(a.rows, a.width)},
                           x.options().dtype(at::kFloat));
       a.partial = partial.data_ptr<float>();
     }
