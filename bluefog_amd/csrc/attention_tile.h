@@ -1,0 +1,280 @@
+// Copyright 2026. Licensed under the Apache License, Version 2.0.
+//
+// What the attention kernels share: matrix fragments, LDS tiles, the search
+// for a workgroup's rows.
+//
+// All products run on 32x32 matrix tiles. A fragment is 8 values of a lane: of
+// row (or column) lane & 31, at the inner positions 8 * (lane >> 5) ... + 7 of
+// a step of 16. Half-precision types have one instruction for a step
+// (32x32x16); f32 takes eight 32x32x2, of which number i multiplies value i of
+// both halves, which is the same sum in another order. The accumulator holds
+// column lane & 31 and, in register r, row 8 * (r >> 2) + 4 * (lane >> 5) +
+// (r & 3).
+//
+// That accumulator is the next product's operand as it stands: eight of its
+// registers are the inner positions {4 half ... + 3, 8 + 4 half ... + 3} of a
+// step of 16, and the other operand is read in the same order (read_columns).
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "convert.h"
+#include "transformer_kernels.h"
+
+namespace bf_attn {
+
+typedef float Acc __attribute__((ext_vector_type(16)));
+
+template <typename T>
+struct FragOf {
+  typedef T type __attribute__((ext_vector_type(8)));
+};
+template <typename T>
+using Frag = typename FragOf<T>::type;
+
+__device__ __forceinline__ Acc mma(Frag<__bf16> a, Frag<__bf16> b, Acc c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ Acc mma(Frag<_Float16> a, Frag<_Float16> b, Acc c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ Acc mma(Frag<float> a, Frag<float> b, Acc c) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
+  return c;
+}
+
+// whether a fragment holds an infinity or what is no number
+template <typename F>
+__device__ __forceinline__ int not_finite(F f) {
+  int found = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) found |= !(fabsf(static_cast<float>(f[i])) < INFINITY);
+  return found;
+}
+
+// inner position of accumulator register r
+__device__ __forceinline__ int row_of(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
+
+// ---------------------------------------------------------------------------
+// LDS tiles: ROWS rows of DP columns, 16-byte chunks, chunk c of row r at
+// c ^ swizzle(r). Eight neighbouring rows' chunks lie in different banks (a
+// fragment of rows), and so do the chunk pairs of four (a fragment of columns).
+// ---------------------------------------------------------------------------
+
+template <typename T, int ROWS, int DP, int THREADS, bool VEC>
+struct Tile {
+  static constexpr int kEach = 16 / sizeof(T);  // values of a chunk
+  static constexpr int kChunks = DP / kEach;
+  static constexpr int kRowBytes = DP * sizeof(T);
+  static constexpr int kBytes = ROWS * kRowBytes;
+
+  static __device__ __forceinline__ int swizzle(int r) {
+    return kChunks == 8 ? (((r >> 1) & 3) << 1) | ((r >> 3) & 1) : ((r & 7) << 1) | ((r >> 3) & 1);
+  }
+  static __device__ __forceinline__ int at(int row, int chunk) {
+    return row * kRowBytes + ((chunk ^ swizzle(row)) << 4);
+  }
+
+  // Rows first .. first + ROWS - 1 of a matrix into the tile, without a
+  // register: a wave's load fills 1024 bytes, and each lane picks the chunk
+  // that belongs there. Rows behind `last` repeat it (they are masked where
+  // they would count, and hold nothing that their sequence does not). Columns
+  // behind dim stay as they are: cleared once.
+  static __device__ __forceinline__ void load(char* lds, const T* base, long stride, int first, int last, int dim) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    if constexpr (VEC) {
+#pragma unroll
+      for (int n = 0; n < kBytes / 1024 / (THREADS / 64); ++n) {
+        const int block = n * (THREADS / 64) + wave;
+        const int off = block * 1024 + lane * 16;
+        const int row = off / kRowBytes, chunk = ((off % kRowBytes) >> 4) ^ swizzle(row);
+        const T* from = base + static_cast<long>(min(first + row, last)) * stride + chunk * kEach;
+        if (chunk * kEach < dim)
+          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                           (__attribute__((address_space(3))) void*)(lds + block * 1024), 16, 0, 0);
+      }
+    } else {
+      for (int i = threadIdx.x; i < ROWS * DP; i += THREADS) {
+        const int row = i / DP, c = i % DP;
+        if (c < dim)
+          *reinterpret_cast<T*>(lds + at(row, c / kEach) + (c % kEach) * sizeof(T)) =
+              base[static_cast<long>(min(first + row, last)) * stride + c];
+      }
+    }
+  }
+
+  static __device__ __forceinline__ void clear(char* lds, int bytes) {
+    for (int i = threadIdx.x * 16; i < bytes; i += THREADS * 16) *reinterpret_cast<uint4*>(lds + i) = uint4{0, 0, 0, 0};
+  }
+
+  // fragment of row `row`, inner positions = columns of step `step`
+  static __device__ __forceinline__ Frag<T> read_row(const char* lds, int row, int step, int half) {
+    Frag<T> f;
+    if constexpr (sizeof(T) == 2) {
+      f = *reinterpret_cast<const Frag<T>*>(lds + at(row, step * 2 + half));
+    } else {
+      typedef float F4 __attribute__((ext_vector_type(4)));
+      const F4 x = *reinterpret_cast<const F4*>(lds + at(row, step * 4 + half * 2));
+      const F4 y = *reinterpret_cast<const F4*>(lds + at(row, step * 4 + half * 2 + 1));
+      f = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    return f;
+  }
+
+  // fragment of column 32 * dt + (lane & 31), inner positions = rows
+  // base + {4 half .. + 3, 8 + 4 half .. + 3}
+  static __device__ __forceinline__ Frag<T> read_columns(const char* lds, int base, int dt, int lane) {
+    const int half = lane >> 5;
+    Frag<T> f;
+    if constexpr (sizeof(T) == 2) {
+      // the transposing read: sixteen lanes give the addresses of 4 rows of 16
+      // values, four to a lane, and lane i gets column i of the four rows
+      typedef short S4 __attribute__((ext_vector_type(4)));
+      const int row = base + 4 * half + ((lane & 15) >> 2);
+      const int c = dt * 32 + (lane & 16) + (lane & 3) * 4;
+      S4 part[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        part[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) S4*)(lds + at(row + 8 * k, c / 8) + (c % 8) * 2));
+      __builtin_memcpy(&f, part, sizeof(f));
+    } else {
+      const int c = dt * 32 + (lane & 31);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        f[j] = *reinterpret_cast<const T*>(lds + at(base + row_of(j, half), c / kEach) + (c % kEach) * sizeof(T));
+    }
+    return f;
+  }
+};
+
+// all of a wave's loads into LDS have landed, and everybody's
+__device__ __forceinline__ void loads_done() {
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  __syncthreads();
+}
+
+// fragment of a row in memory, columns of step `step`; 0 behind dim
+template <bool VEC, typename T>
+__device__ __forceinline__ Frag<T> load_row(const T* row, int step, int half, int dim) {
+  Frag<T> f;
+  const int c = step * 16 + half * 8;
+  if (VEC && c < dim) {
+    if (sizeof(T) == 4 && dim - c < 8) {  // f32: four of eight
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = i < 4 ? row[c + i] : static_cast<T>(0.f);
+    } else {
+      __builtin_memcpy(&f, row + c, sizeof(f));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = !VEC && c + i < dim ? row[c + i] : static_cast<T>(0.f);
+  }
+  return f;
+}
+
+// accumulators [columns of the row on 32 * tiles][one row a lane] times f into
+// memory: 16 bytes a lane. The halves hold quads of columns; a swap gives each
+// eight in a row.
+template <bool VEC, typename T, int TILES>
+__device__ __forceinline__ void store_row(T* row, Acc (&acc)[TILES], float f, int half, int dim, bool inside) {
+#pragma unroll
+  for (int dt = 0; dt < TILES; ++dt)
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // lower half keeps its first quad and takes the upper's, the upper
+        // half keeps its second and takes the lower's
+        const float a = acc[dt][s * 8 + i] * f, b = acc[dt][s * 8 + 4 + i] * f;
+        const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+        x[i] = __uint_as_float(both[0]);
+        x[4 + i] = __uint_as_float(both[1]);
+      }
+      const int c = dt * 32 + s * 16 + half * 8;
+      if (!inside) continue;
+      T t[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] = static_cast<T>(x[i]);
+      if (VEC && c + 8 <= dim) {
+        __builtin_memcpy(row + c, t, sizeof(t));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (c + i < dim) row[c + i] = t[i];
+      }
+    }
+}
+
+__device__ __forceinline__ float swap_halves(float x) {
+  const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return (threadIdx.x & 32) ? __uint_as_float(both[0]) : __uint_as_float(both[1]);
+}
+
+// ---------------------------------------------------------------------------
+// Which rows a workgroup has. The sequences' tiles of `size` rows are numbered
+// through, and so are those of the rows behind the last sequence (`seq` ==
+// seqs then). Every wave searches by itself: lane i counts the tiles of
+// `chunk` sequences, the first lane whose running count exceeds the number has
+// it, and where chunk > 1 the same once more inside. Bounds that are not
+// ordered or leave [0, rows] are cut to it, so that no access leaves the
+// tensors.
+// ---------------------------------------------------------------------------
+
+struct Work {
+  int begin, len;  // rows of the sequence
+  int seq, tile;   // tile inside it
+  int tiles;       // of the sequence
+  bool any;
+};
+
+__device__ __forceinline__ int2 bounds_of(const BfAttnArgs& a, int seq) {
+  int begin = min(max(a.cu[seq], 0), a.rows);
+  int end = seq < a.seqs ? min(max(a.cu[seq + 1], begin), a.rows) : a.rows;
+  return make_int2(begin, end);
+}
+
+__device__ __forceinline__ Work find_tile(const BfAttnArgs& a, int number, int size) {
+  const int lane = threadIdx.x & 63, n = a.seqs + 1;
+  Work w{};
+  int first = 0, count = n, chunk = (n + 63) / 64;
+  while (true) {
+    int mine = 0;
+    for (int i = 0; i < chunk; ++i) {
+      const int s = first + lane * chunk + i;
+      if (lane * chunk + i < count) {
+        const int2 b = bounds_of(a, s);
+        mine += (b.y - b.x + size - 1) / size;
+      }
+    }
+    int upto = mine;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int x = __shfl_up(upto, off, 64);
+      if (lane >= off) upto += x;
+    }
+    const unsigned long long past = __ballot(upto > number);
+    if (!past) return w;
+    const int pick = __ffsll(past) - 1;
+    number -= __shfl(upto - mine, pick, 64);
+    first += pick * chunk;
+    if (chunk == 1) break;
+    count = min(chunk, count - pick * chunk);
+    chunk = (count + 63) / 64;
+  }
+  w.seq = __builtin_amdgcn_readfirstlane(first);
+  w.tile = __builtin_amdgcn_readfirstlane(number);
+  const int2 b = bounds_of(a, w.seq);
+  w.begin = b.x;
+  w.len = b.y - b.x;
+  w.tiles = (w.len + size - 1) / size;
+  w.any = true;
+  return w;
+}
+
+// tiles of `size` rows that any bounds can have, the rows behind included
+inline long most_tiles(const BfAttnArgs& a, int size) { return a.rows / size + a.seqs + 1; }
+
+}  // namespace bf_attn

@@ -468,23 +468,29 @@ __global__ __launch_bounds__(256) void norm_param_wide_k(BfNormArgs a) {
   store8(out + a.width, n, db);
 }
 
-// the partial sums [slots][2][width] into dw and db. 64 columns to a workgroup,
-// the slots over its 16 waves; every sum has a fixed order.
-template <typename TX>
+// the partial sums [slots][2][width] into dw and db: COLUMNS of them to a
+// workgroup, the slots over its other lanes; every sum has a fixed order.
+// Narrow rows take 16 columns, so that there are workgroups enough (768 columns
+// of 1024 slots: 4.7 us, with 64 columns 7.4), wide ones 64, whole lines of
+// 256 bytes (8192 of 512: 7.7 us, with 16 columns 14.1).
+template <typename TX, int COLUMNS>
 __global__ __launch_bounds__(1024) void norm_fold_k(BfNormArgs a, int slots) {
-  __shared__ float lds[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long i = static_cast<long>(blockIdx.x) * 64 + lane, n = 2L * a.width;
+  constexpr int kParts = 1024 / COLUMNS;
+  __shared__ float lds[kParts][COLUMNS];
+  const int column = threadIdx.x % COLUMNS, part = threadIdx.x / COLUMNS;
+  const long i = static_cast<long>(blockIdx.x) * COLUMNS + column, n = 2L * a.width;
   float s = 0.f;
   if (i < n) {
-#pragma unroll 4
-    for (int k = wave; k < slots; k += 16) s += a.partial[k * n + i];
+#pragma unroll 8
+    for (int k = part; k < slots; k += kParts) s += a.partial[k * n + i];
   }
-  lds[wave][lane] = s;
-  __syncthreads();
-  if (wave || i >= n) return;
-#pragma unroll
-  for (int k = 1; k < 16; ++k) s += lds[k][lane];
+  lds[part][column] = s;
+  for (int half = kParts / 2; half > 0; half /= 2) {
+    __syncthreads();
+    if (part < half) lds[part][column] += lds[part + half][column];
+  }
+  if (part || i >= n) return;
+  s = lds[0][column];
   void* to = i < a.width ? a.dweight : a.dbias;
   const long c = i < a.width ? i : i - a.width;
   if (!to) return;
@@ -594,7 +600,10 @@ struct Bwd {
     }
     if (hipError_t e = hipGetLastError()) return e;
     if (!a.partial) return hipSuccess;
-    hipLaunchKernelGGL(norm_fold_k<TX>, dim3((2L * a.width + 63) / 64), dim3(1024), 0, stream, a, slots);
+    if (a.width < 4096)
+      hipLaunchKernelGGL((norm_fold_k<TX, 16>), dim3((2L * a.width + 15) / 16), dim3(1024), 0, stream, a, slots);
+    else
+      hipLaunchKernelGGL((norm_fold_k<TX, 64>), dim3((2L * a.width + 63) / 64), dim3(1024), 0, stream, a, slots);
     return hipGetLastError();
   }
 };
