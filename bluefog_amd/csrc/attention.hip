@@ -14,52 +14,7 @@
 
 namespace {
 
-constexpr int kWaves = 4;
 constexpr float kLog2e = 1.4426950408889634f;
-
-__device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
-  return x;
-}
-
-// the sequence that holds a row: [begin, end), empty if none does. Bounds that
-// are not ordered or leave [0, rows] are cut to it, so no access leaves the
-// tensors.
-__device__ __forceinline__ int2 sequence_of(const BfAttnArgs& a, int row) {
-  int lo = 0, hi = a.seqs;  // last b with cu[b] <= row
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.cu[mid] <= row) lo = mid; else hi = mid - 1;
-  }
-  if (lo >= a.seqs) return make_int2(0, 0);
-  const int begin = max(a.cu[lo], 0), end = min(a.cu[lo + 1], a.rows);
-  return row >= begin && row < end ? make_int2(begin, end) : make_int2(0, 0);
-}
-
-// One wave to a row and head; lane l holds columns l and l + 64.
-template <typename T>
-struct Row {
-  float x[2];
-  __device__ Row() : x{0.f, 0.f} {}
-  __device__ void load(const void* base, long at, int dim, int lane) {
-    const T* p = static_cast<const T*>(base) + at;
-    x[0] = lane < dim ? bf_to_float(p[lane]) : 0.f;
-    x[1] = lane + 64 < dim ? bf_to_float(p[lane + 64]) : 0.f;
-  }
-  __device__ void store(void* base, long at, int dim, int lane, float f) const {
-    T* p = static_cast<T*>(base) + at;
-    if (lane < dim) p[lane] = static_cast<T>(x[0] * f);
-    if (lane + 64 < dim) p[lane + 64] = static_cast<T>(x[1] * f);
-  }
-  __device__ float dot(const Row& o) const {
-    return wave_sum(x[0] * o.x[0] + x[1] * o.x[1]);
-  }
-  __device__ void add(const Row& o, float f) {
-    x[0] += f * o.x[0];
-    x[1] += f * o.x[1];
-  }
-};
 
 using namespace bf_attn;
 
@@ -104,6 +59,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_k(BfAttnArgs a) {
   const T* k = static_cast<const T*>(a.k) + static_cast<long>(w.begin) * a.k_row + g * a.k_head;
   const T* v = static_cast<const T*>(a.v) + static_cast<long>(w.begin) * a.v_row + g * a.v_head;
   const int last = w.len - 1, keys = a.causal ? min(w.len, q0 + kQ) : w.len;
+  const int seen = a.causal ? min(w.len, qi + 1) : w.len;  // keys of the lane's row
   if (a.dim < DP) {
     KV::clear(&lds[0][0][0], sizeof(lds));
     __syncthreads();
@@ -137,7 +93,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_k(BfAttnArgs a) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int j = k0 + u * 32 + row_of(r, half);
-            if (j >= w.len || (a.causal && j > qi)) s[u][r] = -INFINITY;
+            s[u][r] = j < seen ? s[u][r] : -INFINITY;
           }
       }
       float top = s[0][0];
@@ -192,17 +148,17 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_k(BfAttnArgs a) {
           Acc count{};
 #pragma unroll
           for (int u = 0; u < BN / 16; ++u) {
-            Frag<T> f = KV::read_columns(lds[buf][1], u * 16, i, lane), bad, seen;
+            Frag<T> f = KV::read_columns(lds[buf][1], u * 16, i, lane), bad, sees;
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
               const int j = k0 + u * 16 + row_of(r, half);
               const bool fine = fabsf(static_cast<float>(f[r])) < INFINITY;
               bad[r] = static_cast<T>(fine ? 0.f : 1.f);
               f[r] = fine ? f[r] : static_cast<T>(0.f);
-              seen[r] = static_cast<T>(j < w.len && j <= qi ? 1.f : 0.f);
+              sees[r] = static_cast<T>(j < seen ? 1.f : 0.f);
             }
             o[i] = mma(f, p[u], o[i]);
-            count = mma(bad, seen, count);
+            count = mma(bad, sees, count);
           }
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[i][r] = count[r] > 0.f ? NAN : o[i][r];
@@ -216,64 +172,290 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_k(BfAttnArgs a) {
   if (a.lse && inside && half == 0) a.lse[static_cast<long>(h) * a.rows + row] = m * c + log2f(l);
 }
 
-template <typename T>
-__global__ __launch_bounds__(kWaves * 64) void attn_dq_k(BfAttnArgs a) {
-  const long unit = static_cast<long>(blockIdx.x) * kWaves + threadIdx.x / 64;
-  if (unit >= static_cast<long>(a.rows) * a.heads) return;
-  const int lane = threadIdx.x & 63;
-  const int row = static_cast<int>(unit / a.heads), h = static_cast<int>(unit % a.heads);
-  const int g = h / (a.heads / a.kv_heads);
-  const int2 seq = sequence_of(a, row);
-  const BfKey key = a.drop.threshold ? bf_key(a.drop) : BfKey{0, 0};
-  const long at = static_cast<long>(h) * a.rows + row;
-  Row<T> q, o, go, k, v, dq;
-  q.load(a.q, row * a.q_row + h * a.q_head, a.dim, lane);
-  go.load(a.dout, row * a.do_row + h * a.do_head, a.dim, lane);
-  o.load(a.out, unit * a.dim, a.dim, lane);
-  const float delta = go.dot(o), lse = a.lse[at];
-  if (lane == 0) a.delta[at] = delta;
-  const int stop = a.causal ? min(seq.y, row + 1) : seq.y;
-  // a row that sees one key has P = 1 whatever its score: dS is 0, not the
-  // rounding of dP - delta
-  for (int j = seq.x; j < stop && stop - seq.x > 1; ++j) {
-    k.load(a.k, j * a.k_row + g * a.k_head, a.dim, lane);
-    v.load(a.v, j * a.v_row + g * a.v_head, a.dim, lane);
-    const float p = exp2f(q.dot(k) * a.scale * kLog2e - lse);
-    const float keep = a.drop.threshold ? bf_attn_keep(h, row, j - seq.x, a.drop, key) : 1.f;
-    const float dp = keep != 0.f ? keep * go.dot(v) : 0.f;
-    dq.add(k, p * (dp - delta));
-  }
-  dq.store(a.dq, unit * a.dim, a.dim, lane, a.scale);
-}
+// ---------------------------------------------------------------------------
+// backward, dq: the same loop as forward, with dP^T = v dO^T beside S^T, and
+// dq^T = k^T dS^T. Its first act is delta, which the other kernel reads.
+//
+// f16 would lose small dS and overflow with large ones, whatever dO's size.
+// Its dS is held times a power of two of its own for each lane's row (or key),
+// lowered with the accumulators when a tile brings a larger value.
+// ---------------------------------------------------------------------------
 
 template <typename T>
-__global__ __launch_bounds__(kWaves * 64) void attn_dkv_k(BfAttnArgs a) {
-  const long unit = static_cast<long>(blockIdx.x) * kWaves + threadIdx.x / 64;
-  if (unit >= static_cast<long>(a.rows) * a.kv_heads) return;
-  const int lane = threadIdx.x & 63;
-  const int j = static_cast<int>(unit / a.kv_heads), g = static_cast<int>(unit % a.kv_heads);
-  const int group = a.heads / a.kv_heads;
-  const int2 seq = sequence_of(a, j);
-  const BfKey key = a.drop.threshold ? bf_key(a.drop) : BfKey{0, 0};
-  Row<T> q, go, k, v, dk, dv;
-  k.load(a.k, j * a.k_row + g * a.k_head, a.dim, lane);
-  v.load(a.v, j * a.v_row + g * a.v_head, a.dim, lane);
-  for (int h = g * group; h < (g + 1) * group; ++h)
-    for (int row = a.causal ? max(j, seq.x) : seq.x; row < seq.y; ++row) {
-      const long at = static_cast<long>(h) * a.rows + row;
-      q.load(a.q, row * a.q_row + h * a.q_head, a.dim, lane);
-      go.load(a.dout, row * a.do_row + h * a.do_head, a.dim, lane);
-      const float p = exp2f(q.dot(k) * a.scale * kLog2e - a.lse[at]);
-      const float keep = a.drop.threshold ? bf_attn_keep(h, row, j - seq.x, a.drop, key) : 1.f;
-      if (keep != 0.f) dv.add(go, p * keep);
-      const int sees = a.causal ? row + 1 - seq.x : seq.y - seq.x;
-      if (sees > 1) {
-        const float dp = keep != 0.f ? keep * go.dot(v) : 0.f;
-        dk.add(q, p * (dp - a.delta[at]));
+constexpr bool kScaled = false;
+template <>
+constexpr bool kScaled<_Float16> = true;
+// power of two that P is held times in the backward pass
+template <typename T>
+constexpr float kPower = kScaled<T> ? 12.f : 0.f;
+
+template <int TILES>
+__device__ __forceinline__ void rescale(Acc (&acc)[TILES], float& factor, const float* x) {
+  float top = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(x[r]));
+  top = fmaxf(top, swap_halves(top));
+  const bool lower = top < INFINITY && top > 0.f && (factor == 0.f || top * factor > 32768.f);
+  if (!__any(lower)) return;
+  if (lower) {
+    int e;
+    frexpf(top, &e);
+    const float next = ldexpf(1.f, min(14 - e, 100));
+    const float by = factor == 0.f ? 1.f : next / factor;
+    factor = next;
+#pragma unroll
+    for (int i = 0; i < TILES; ++i) acc[i] *= by;
+  }
+}
+
+template <typename T, int DP, bool VEC, bool DROP>
+__global__ __launch_bounds__(256, 2) void attn_dq_k(BfAttnArgs a) {
+  constexpr int kQ = 128, BN = kKeys<T>, kSub = BN / 32, kSteps = DP / 16, kDT = DP / 32;
+  typedef Tile<T, BN, DP, 256, VEC> KV;
+  __shared__ __align__(1024) char lds[2][2][KV::kBytes];
+  const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
+  const int h = blockIdx.x % a.heads, g = h / (a.heads / a.kv_heads);
+  Work w = find_tile(a, blockIdx.x / a.heads, kQ);
+  if (!w.any) return;
+  if (a.causal) w.tile = w.tiles - 1 - w.tile;
+  const int q0 = w.tile * kQ, qw = q0 + wave * 32, qi = qw + (lane & 31);
+  const bool inside = qi < w.len;
+  const long row = w.begin + min(qi, w.len - 1), at = static_cast<long>(h) * a.rows + row;
+  T* out = static_cast<T*>(a.dq) + (row * a.heads + h) * a.dim;
+  Acc dq[kDT];
+#pragma unroll
+  for (int i = 0; i < kDT; ++i) dq[i] = Acc{};
+  if (w.seq == a.seqs) {  // behind the last sequence
+    store_row<VEC>(out, dq, 0.f, half, a.dim, inside);
+    return;
+  }
+  const T* k = static_cast<const T*>(a.k) + static_cast<long>(w.begin) * a.k_row + g * a.k_head;
+  const T* v = static_cast<const T*>(a.v) + static_cast<long>(w.begin) * a.v_row + g * a.v_head;
+  const int last = w.len - 1, keys = a.causal ? min(w.len, q0 + kQ) : w.len;
+  if (a.dim < DP) {
+    KV::clear(&lds[0][0][0], sizeof(lds));
+    __syncthreads();
+  }
+  KV::load(lds[0][0], k, a.k_row, 0, last, a.dim);
+  KV::load(lds[0][1], v, a.v_row, 0, last, a.dim);
+  Frag<T> qf[kSteps], gf[kSteps];
+  float delta = 0.f;
+  {
+    const T* q = static_cast<const T*>(a.q) + row * a.q_row + h * a.q_head;
+    const T* go = static_cast<const T*>(a.dout) + row * a.do_row + h * a.do_head;
+    const T* o = static_cast<const T*>(a.out) + (row * a.heads + h) * a.dim;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      qf[s] = load_row<VEC>(q, s, half, a.dim);
+      gf[s] = load_row<VEC>(go, s, half, a.dim);
+      const Frag<T> of = load_row<VEC>(o, s, half, a.dim);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) delta += static_cast<float>(gf[s][i]) * static_cast<float>(of[i]);
+    }
+    delta += swap_halves(delta);
+  }
+  if (inside && half == 0) a.delta[at] = delta;
+  const BfKey key = DROP ? bf_key(a.drop) : BfKey{0, 0};
+  const float c = a.scale * kLog2e, lse = a.lse[at] - kPower<T>;
+  // keys of the lane's row that have a dS: a row that sees one key has P = 1
+  // whatever its score, and dS is 0, not the rounding of dP - delta
+  int seen = a.causal ? min(w.len, qi + 1) : w.len;
+  seen = seen == 1 ? 0 : seen;
+  float factor = 0.f;  // f16: what dS is held times
+  loads_done();
+  for (int k0 = 0, buf = 0; k0 < keys; k0 += BN, buf ^= 1) {
+    if (k0 + BN < keys) {
+      KV::load(lds[buf ^ 1][0], k, a.k_row, k0 + BN, last, a.dim);
+      KV::load(lds[buf ^ 1][1], v, a.v_row, k0 + BN, last, a.dim);
+    }
+    if (qw < w.len && !(a.causal && k0 > qw + 31)) {
+      const bool masked = k0 + BN > w.len || (a.causal && (k0 + BN - 1 > qw || qw == 0));
+#pragma unroll
+      for (int u = 0; u < kSub; ++u) {
+        Acc s{}, dp{};
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) s = mma(KV::read_row(lds[buf][0], u * 32 + (lane & 31), i, half), qf[i], s);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) dp = mma(KV::read_row(lds[buf][1], u * 32 + (lane & 31), i, half), gf[i], dp);
+        float ds[16];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          uint4 bits;
+          if (DROP)
+            bits = bf_philox((k0 / 16 + u * 2 + t) * 2 + half, static_cast<uint32_t>(row), h, a.drop.offset, key);
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            float x = dp[t * 8 + r];
+            if (DROP) x = bf_half(bits, r) >= a.drop.threshold ? x * a.drop.scale : 0.f;
+            ds[t * 8 + r] = __builtin_amdgcn_exp2f(s[t * 8 + r] * c - lse) * (x - delta);
+          }
+        }
+        if (masked) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int j = k0 + u * 32 + row_of(r, half);
+            ds[r] = j < seen ? ds[r] : 0.f;
+          }
+        }
+        if constexpr (kScaled<T>) {
+          rescale(dq, factor, ds);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) ds[r] *= factor;
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          Frag<T> f;
+#pragma unroll
+          for (int r = 0; r < 8; ++r) f[r] = static_cast<T>(ds[t * 8 + r]);
+#pragma unroll
+          for (int i = 0; i < kDT; ++i) dq[i] = mma(KV::read_columns(lds[buf][0], u * 32 + t * 16, i, lane), f, dq[i]);
+        }
       }
     }
-  dk.store(a.dk, unit * a.dim, a.dim, lane, a.scale);
-  dv.store(a.dv, unit * a.dim, a.dim, lane, 1.f);
+    loads_done();
+  }
+  const float f = kScaled<T> ? (factor == 0.f ? 1.f : exp2f(-kPower<T>) / factor) : 1.f;
+  store_row<VEC>(out, dq, a.scale * f, half, a.dim, inside);
+}
+
+// ---------------------------------------------------------------------------
+// backward, dk and dv: a wave has 32 keys, one to a lane of each half, and goes
+// over the queries that see them, head by head of the group. S = q k^T and dP
+// lie with a key's queries in the registers of its lane pair, so that P and dS
+// are the operands of dv^T = dO^T P and dk^T = q^T dS as they stand.
+// ---------------------------------------------------------------------------
+
+template <typename T, int DP, bool VEC, bool DROP>
+__global__ __launch_bounds__(256, 2) void attn_dkv_k(BfAttnArgs a) {
+  constexpr int kK = 128, BM = kKeys<T>, kSub = BM / 32, kSteps = DP / 16, kDT = DP / 32;
+  typedef Tile<T, BM, DP, 256, VEC> QG;
+  __shared__ __align__(1024) char lds[2][2][QG::kBytes];
+  __shared__ __align__(16) float stat[2][2][BM];       // lse and delta of the tile's queries
+  __shared__ __align__(16) uint32_t kept[4][DROP ? 32 : 4];  // a wave's mask: a query's 32 keys to a word
+  const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
+  const int g = blockIdx.x % a.kv_heads, group = a.heads / a.kv_heads;
+  const Work w = find_tile(a, blockIdx.x / a.kv_heads, kK);
+  if (!w.any) return;
+  const int j0 = w.tile * kK, jw = j0 + wave * 32, ji = jw + (lane & 31);
+  const bool inside = ji < w.len;
+  const long row = w.begin + min(ji, w.len - 1), out = (row * a.kv_heads + g) * a.dim;
+  Acc dk[kDT], dv[kDT];
+#pragma unroll
+  for (int i = 0; i < kDT; ++i) dk[i] = dv[i] = Acc{};
+  if (w.seq == a.seqs) {  // behind the last sequence
+    store_row<VEC>(static_cast<T*>(a.dk) + out, dk, 0.f, half, a.dim, inside);
+    store_row<VEC>(static_cast<T*>(a.dv) + out, dv, 0.f, half, a.dim, inside);
+    return;
+  }
+  Frag<T> kf[kSteps], vf[kSteps];
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    kf[s] = load_row<VEC>(static_cast<const T*>(a.k) + row * a.k_row + g * a.k_head, s, half, a.dim);
+    vf[s] = load_row<VEC>(static_cast<const T*>(a.v) + row * a.v_row + g * a.v_head, s, half, a.dim);
+  }
+  const int last = w.len - 1;
+  const int first = a.causal ? j0 / BM * BM : 0;  // queries in front of the keys see none of them
+  const int from = a.causal ? ji : 0;  // first query that sees the lane's key
+  const int from_ds = a.causal ? max(ji, 1) : w.len == 1 ? 1 : 0;  // and has another: with one key dS is 0
+  const int total = (w.len - first + BM - 1) / BM * group;
+  if (a.dim < DP) {
+    QG::clear(&lds[0][0][0], sizeof(lds));
+    __syncthreads();
+  }
+  const auto fetch = [&](int h, int i0, int buf) {
+    const T* q = static_cast<const T*>(a.q) + static_cast<long>(w.begin) * a.q_row + h * a.q_head;
+    const T* go = static_cast<const T*>(a.dout) + static_cast<long>(w.begin) * a.do_row + h * a.do_head;
+    QG::load(lds[buf][0], q, a.q_row, i0, last, a.dim);
+    QG::load(lds[buf][1], go, a.do_row, i0, last, a.dim);
+    if (wave < 2 && lane < BM) {
+      const float* from = (wave ? a.delta : a.lse) + static_cast<long>(h) * a.rows + w.begin + min(i0 + lane, last);
+      load_to_lds<4>(from, stat[buf][wave]);
+    }
+  };
+  const BfKey key = DROP ? bf_key(a.drop) : BfKey{0, 0};
+  const float c = a.scale * kLog2e;
+  float factor = 0.f;
+  int h = g * group, i0 = first;  // head and queries of a step, and of the next
+  fetch(h, i0, 0);
+  loads_done();
+  for (int n = 0, buf = 0, next_h, next_i0; n < total; ++n, buf ^= 1, h = next_h, i0 = next_i0) {
+    next_h = h, next_i0 = i0 + BM;
+    if (next_i0 >= w.len) ++next_h, next_i0 = first;
+    if (n + 1 < total) fetch(next_h, next_i0, buf ^ 1);
+    if (jw < w.len && !(a.causal && i0 + BM - 1 < jw)) {
+      const bool masked = i0 + BM > w.len || (a.causal && (i0 < jw + 31 || i0 == 0)) || w.len == 1;
+#pragma unroll
+      for (int u = 0; u < kSub; ++u) {
+        Acc s{}, dp{};
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) s = mma(QG::read_row(lds[buf][0], u * 32 + (lane & 31), i, half), kf[i], s);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) dp = mma(QG::read_row(lds[buf][1], u * 32 + (lane & 31), i, half), vf[i], dp);
+        if (DROP) {
+          // the lane's share of a query's mask, as the forward pass has it
+          uint32_t bits = 0;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const uint4 x = bf_philox((jw / 16 + t) * 2 + half, static_cast<uint32_t>(w.begin + i0 + u * 32 + (lane & 31)),
+                                      h, a.drop.offset, key);
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+              bits |= (bf_half(x, r) >= a.drop.threshold ? 1u : 0u) << (t * 16 + 8 * (r >> 2) + (r & 3));
+          }
+          bits <<= 4 * half;
+          bits |= __float_as_uint(swap_halves(__uint_as_float(bits)));
+          if (half == 0) kept[wave][lane] = bits;
+        }
+        float p[16], ds[16];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const float4 lse = *reinterpret_cast<const float4*>(&stat[buf][0][u * 32 + t * 8 + half * 4]);
+          const float4 delta = *reinterpret_cast<const float4*>(&stat[buf][1][u * 32 + t * 8 + half * 4]);
+          uint4 m = uint4{0, 0, 0, 0};
+          if (DROP) m = *reinterpret_cast<const uint4*>(&kept[wave][t * 8 + half * 4]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float l = r == 0 ? lse.x : r == 1 ? lse.y : r == 2 ? lse.z : lse.w;
+            const float d = r == 0 ? delta.x : r == 1 ? delta.y : r == 2 ? delta.z : delta.w;
+            const uint32_t word = r == 0 ? m.x : r == 1 ? m.y : r == 2 ? m.z : m.w;
+            const float x = __builtin_amdgcn_exp2f(s[t * 4 + r] * c - (l - kPower<T>));
+            const bool keep = !DROP || (word >> (lane & 31)) & 1;
+            const float y = keep ? (DROP ? dp[t * 4 + r] * a.drop.scale : dp[t * 4 + r]) : 0.f;
+            p[t * 4 + r] = keep ? x : 0.f;
+            ds[t * 4 + r] = x * (y - d);
+          }
+        }
+        if (masked) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int i = i0 + u * 32 + row_of(r, half);
+            p[r] = i >= from && i < w.len ? p[r] : 0.f;
+            ds[r] = i >= from_ds && i < w.len ? ds[r] : 0.f;
+          }
+        }
+        if constexpr (kScaled<T>) {
+          rescale(dk, factor, ds);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) ds[r] *= factor;
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          Frag<T> pf, df;
+#pragma unroll
+          for (int r = 0; r < 8; ++r) pf[r] = static_cast<T>(p[t * 8 + r]), df[r] = static_cast<T>(ds[t * 8 + r]);
+#pragma unroll
+          for (int i = 0; i < kDT; ++i) {
+            dv[i] = mma(QG::read_columns(lds[buf][1], u * 32 + t * 16, i, lane), pf, dv[i]);
+            dk[i] = mma(QG::read_columns(lds[buf][0], u * 32 + t * 16, i, lane), df, dk[i]);
+          }
+        }
+      }
+    }
+    loads_done();
+  }
+  const float power = exp2f(-kPower<T>), f = kScaled<T> ? (factor == 0.f ? 1.f : power / factor) : 1.f;
+  store_row<VEC>(static_cast<T*>(a.dk) + out, dk, a.scale * f, half, a.dim, inside);
+  store_row<VEC>(static_cast<T*>(a.dv) + out, dv, power * (DROP ? a.drop.scale : 1.f), half, a.dim, inside);
 }
 
 template <typename T, int DP, bool VEC>
@@ -291,14 +473,25 @@ hipError_t fwd(const BfAttnArgs& a, hipStream_t stream) {
   return a.dim <= 64 ? fwd<T, 64, true>(a, stream) : fwd<T, 128, true>(a, stream);
 }
 
+template <typename T, int DP, bool VEC, bool DROP>
+hipError_t bwd(const BfAttnArgs& a, bool need_dkv, hipStream_t stream) {
+  const long groups = most_tiles(a, 128) * a.heads, shared = most_tiles(a, 128) * a.kv_heads;
+  if (groups > 0x7FFFFFFF) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((attn_dq_k<T, DP, VEC, DROP>), dim3(groups), dim3(256), 0, stream, a);
+  if (hipError_t e = hipGetLastError()) return e;
+  if (need_dkv) hipLaunchKernelGGL((attn_dkv_k<T, DP, VEC, DROP>), dim3(shared), dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+template <typename T, int DP, bool VEC>
+hipError_t bwd(const BfAttnArgs& a, bool need_dkv, hipStream_t stream) {
+  return a.drop.threshold ? bwd<T, DP, VEC, true>(a, need_dkv, stream) : bwd<T, DP, VEC, false>(a, need_dkv, stream);
+}
+
 template <typename T>
 hipError_t bwd(const BfAttnArgs& a, bool need_dkv, hipStream_t stream) {
-  const long units = static_cast<long>(a.rows) * a.heads, shared = static_cast<long>(a.rows) * a.kv_heads;
-  hipLaunchKernelGGL(attn_dq_k<T>, dim3((units + kWaves - 1) / kWaves), dim3(kWaves * 64), 0, stream, a);
-  if (hipError_t e = hipGetLastError()) return e;
-  if (!need_dkv) return hipSuccess;
-  hipLaunchKernelGGL(attn_dkv_k<T>, dim3((shared + kWaves - 1) / kWaves), dim3(kWaves * 64), 0, stream, a);
-  return hipGetLastError();
+  if (!a.vec) return a.dim <= 64 ? bwd<T, 64, false>(a, need_dkv, stream) : bwd<T, 128, false>(a, need_dkv, stream);
+  return a.dim <= 64 ? bwd<T, 64, true>(a, need_dkv, stream) : bwd<T, 128, true>(a, need_dkv, stream);
 }
 
 }  // namespace

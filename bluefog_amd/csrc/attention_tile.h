@@ -56,6 +56,16 @@ __device__ __forceinline__ int not_finite(F f) {
 // inner position of accumulator register r
 __device__ __forceinline__ int row_of(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
 
+// BYTES of each active lane's memory to lds + BYTES * lane, without a register
+template <int BYTES>
+__device__ __forceinline__ void load_to_lds(const void* from, void* lds) {
+  const auto* g = (const __attribute__((address_space(1))) void*)from;
+  auto* l = (__attribute__((address_space(3))) void*)lds;
+  static_assert(BYTES == 4 || BYTES == 16, "a load's size");
+  if constexpr (BYTES == 16) __builtin_amdgcn_global_load_lds(g, l, 16, 0, 0);
+  else __builtin_amdgcn_global_load_lds(g, l, 4, 0, 0);
+}
+
 // ---------------------------------------------------------------------------
 // LDS tiles: ROWS rows of DP columns, 16-byte chunks, chunk c of row r at
 // c ^ swizzle(r). Eight neighbouring rows' chunks lie in different banks (a
@@ -90,9 +100,7 @@ struct Tile {
         const int off = block * 1024 + lane * 16;
         const int row = off / kRowBytes, chunk = ((off % kRowBytes) >> 4) ^ swizzle(row);
         const T* from = base + static_cast<long>(min(first + row, last)) * stride + chunk * kEach;
-        if (chunk * kEach < dim)
-          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
-                                           (__attribute__((address_space(3))) void*)(lds + block * 1024), 16, 0, 0);
+        if (chunk * kEach < dim) load_to_lds<16>(from, lds + block * 1024);
       }
     } else {
       for (int i = threadIdx.x; i < ROWS * DP; i += THREADS) {
