@@ -29,6 +29,11 @@ using namespace bf_attn;
 template <typename T>
 constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;  // keys of a tile
 
+template <int N>
+struct Mode {
+  static constexpr int value = N;
+};
+
 // The accumulators are scaled down only where a maximum has grown by more than
 // this (in powers of two): until then P is at most 2^8, in range of every type.
 constexpr float kSlack = 8.f;
@@ -72,100 +77,120 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_k(BfAttnArgs a) {
   const BfKey key = DROP ? bf_key(a.drop) : BfKey{0, 0};
   const float c = a.scale * kLog2e;
   float m = -INFINITY, l = 0.f;  // of scores without c
-  loads_done();
-  for (int k0 = 0, buf = 0; k0 < keys; k0 += BN, buf ^= 1) {
-    if (k0 + BN < keys) {
-      KV::load(lds[buf ^ 1][0], k, a.k_row, k0 + BN, last, a.dim);
-      KV::load(lds[buf ^ 1][1], v, a.v_row, k0 + BN, last, a.dim);
+  // One tile of keys. MASKED: some of them are not seen by some of the
+  // workgroup's rows. CLEAN: see below.
+  const auto attend = [&](auto mode, int k0, int buf) __attribute__((always_inline)) {
+    constexpr bool MASKED = decltype(mode)::value > 0, CLEAN = decltype(mode)::value > 1;
+    Acc s[kSub];
+#pragma unroll
+    for (int u = 0; u < kSub; ++u) {
+      s[u] = Acc{};
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) s[u] = mma(KV::read_row(lds[buf][0], u * 32 + (lane & 31), i, half), qf[i], s[u]);
     }
-    if (qw < w.len && !(a.causal && k0 > qw + 31)) {
-      Acc s[kSub];
-#pragma unroll
-      for (int u = 0; u < kSub; ++u) {
-        s[u] = Acc{};
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) s[u] = mma(KV::read_row(lds[buf][0], u * 32 + (lane & 31), i, half), qf[i], s[u]);
-      }
-      const bool masked = k0 + BN > w.len || (a.causal && k0 + BN - 1 > qw);
-      if (masked) {
-#pragma unroll
-        for (int u = 0; u < kSub; ++u)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int j = k0 + u * 32 + row_of(r, half);
-            s[u][r] = j < seen ? s[u][r] : -INFINITY;
-          }
-      }
-      float top = s[0][0];
+    if (MASKED) {
 #pragma unroll
       for (int u = 0; u < kSub; ++u)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
-      top = fmaxf(top, swap_halves(top));
-      const bool grow = (top - m) * c > kSlack || m == -INFINITY;
-      if (__any(grow)) {
-        const float grown = grow ? fmaxf(m, top) : m;  // a row's roundings do not depend on other rows
-        const float shrink = m == -INFINITY ? 0.f : exp2f((m - grown) * c);
-        l *= shrink;
+        for (int r = 0; r < 16; ++r) s[u][r] = k0 + u * 32 + row_of(r, half) < seen ? s[u][r] : -INFINITY;
+    }
+    float top = s[0][0];
 #pragma unroll
-        for (int i = 0; i < kDT; ++i) o[i] *= shrink;
-        m = grown;
-      }
-      const float base = m == -INFINITY ? 0.f : m * c;  // all scores so far -inf: P = 0
-      Frag<T> p[BN / 16];
+    for (int u = 0; u < kSub; ++u)
 #pragma unroll
-      for (int u = 0; u < BN / 16; ++u) {
-        uint4 bits;
-        if (DROP) bits = bf_philox((k0 / 16 + u) * 2 + half, static_cast<uint32_t>(row), h, a.drop.offset, key);
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
+    top = fmaxf(top, swap_halves(top));
+    const bool grow = (top - m) * c > kSlack || m == -INFINITY;
+    if (__any(grow)) {
+      const float grown = grow ? fmaxf(m, top) : m;  // a row's roundings do not depend on other rows
+      const float shrink = m == -INFINITY ? 0.f : exp2f((m - grown) * c);
+      l *= shrink;
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          float x = __builtin_amdgcn_exp2f(s[u / 2][(u & 1) * 8 + r] * c - base);
-          l += x;
-          if (DROP) x = bf_half(bits, r) >= a.drop.threshold ? x : 0.f;
-          p[u][r] = static_cast<T>(x);
-        }
-      }
-      // A masked P is 0, and 0 times a value that is no number is none: where a
-      // later key's v holds one, it leaves the product and its column is set
-      // for the rows that see the key.
-      bool spoilt = false;
-      if (masked && a.causal) {
-        int found = 0;
+      for (int i = 0; i < kDT; ++i) o[i] *= shrink;
+      m = grown;
+    }
+    const float base = m == -INFINITY ? 0.f : m * c;  // all scores so far -inf: P = 0
+    Frag<T> p[BN / 16];
 #pragma unroll
-        for (int u = 0; u < BN / 16; ++u)
+    for (int u = 0; u < BN / 16; ++u) {
+      uint4 bits;
+      if (DROP) bits = bf_philox((k0 / 16 + u) * 2 + half, static_cast<uint32_t>(row), h, a.drop.offset, key);
 #pragma unroll
-          for (int i = 0; i < kDT; ++i) found |= not_finite(KV::read_columns(lds[buf][1], u * 16, i, lane));
-        spoilt = __any(found);
-      }
-      if (!spoilt) {
-#pragma unroll
-        for (int u = 0; u < BN / 16; ++u)
-#pragma unroll
-          for (int i = 0; i < kDT; ++i) o[i] = mma(KV::read_columns(lds[buf][1], u * 16, i, lane), p[u], o[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < kDT; ++i) {
-          Acc count{};
-#pragma unroll
-          for (int u = 0; u < BN / 16; ++u) {
-            Frag<T> f = KV::read_columns(lds[buf][1], u * 16, i, lane), bad, sees;
-#pragma unroll
-            for (int r = 0; r < 8; ++r) {
-              const int j = k0 + u * 16 + row_of(r, half);
-              const bool fine = fabsf(static_cast<float>(f[r])) < INFINITY;
-              bad[r] = static_cast<T>(fine ? 0.f : 1.f);
-              f[r] = fine ? f[r] : static_cast<T>(0.f);
-              sees[r] = static_cast<T>(j < seen ? 1.f : 0.f);
-            }
-            o[i] = mma(f, p[u], o[i]);
-            count = mma(bad, sees, count);
-          }
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[i][r] = count[r] > 0.f ? NAN : o[i][r];
-        }
+      for (int r = 0; r < 8; ++r) {
+        float x = __builtin_amdgcn_exp2f(s[u / 2][(u & 1) * 8 + r] * c - base);
+        l += x;
+        if (DROP) x = bf_half(bits, r) >= a.drop.threshold ? x : 0.f;
+        p[u][r] = static_cast<T>(x);
       }
     }
+    if (!CLEAN) {
+#pragma unroll
+      for (int u = 0; u < BN / 16; ++u)
+#pragma unroll
+        for (int i = 0; i < kDT; ++i) o[i] = mma(KV::read_columns(lds[buf][1], u * 16, i, lane), p[u], o[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kDT; ++i) {
+        Acc count{};
+#pragma unroll
+        for (int u = 0; u < BN / 16; ++u) {
+          Frag<T> f = KV::read_columns(lds[buf][1], u * 16, i, lane), bad, sees;
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            const bool fine = fabsf(static_cast<float>(f[r])) < INFINITY;
+            bad[r] = static_cast<T>(fine ? 0.f : 1.f);
+            f[r] = fine ? f[r] : static_cast<T>(0.f);
+            sees[r] = static_cast<T>(k0 + u * 16 + row_of(r, half) < seen ? 1.f : 0.f);
+          }
+          o[i] = mma(f, p[u], o[i]);
+          count = mma(bad, sees, count);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[i][r] = count[r] > 0.f ? NAN : o[i][r];
+      }
+    }
+  };
+  // all tiles, from the one whose load is under way into buffer 0; those that
+  // no row has to mask have a loop of their own
+  const auto all_tiles = [&](auto masked) __attribute__((always_inline)) {
+    const int whole = a.causal ? (q0 + 1) / BN * BN : w.len / BN * BN;
     loads_done();
+    int k0 = 0, buf = 0;
+    const auto next = [&]() __attribute__((always_inline)) {
+      if (k0 + BN >= keys) return;
+      KV::load(lds[buf ^ 1][0], k, a.k_row, k0 + BN, last, a.dim);
+      KV::load(lds[buf ^ 1][1], v, a.v_row, k0 + BN, last, a.dim);
+    };
+    for (; k0 < whole; k0 += BN, buf ^= 1) {
+      next();
+      if (qw < w.len) attend(Mode<0>(), k0, buf);
+      loads_done();
+    }
+    for (; k0 < keys; k0 += BN, buf ^= 1) {
+      next();
+      if (qw < w.len && !(a.causal && k0 > qw + 31)) attend(masked, k0, buf);
+      loads_done();
+    }
+  };
+  all_tiles(Mode<1>());
+  if (a.causal) {
+    // A masked P is 0, and 0 times a value that is no number is none: if a v
+    // of the masked tiles holds one, rows that do not see it have lost their
+    // sum. Once more then, and it leaves the product: its column is set for the
+    // rows that see the key.
+    bool lost = false;
+#pragma unroll
+    for (int i = 0; i < kDT; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) lost |= !(fabsf(o[i][r]) < INFINITY);
+    if (__syncthreads_or(lost)) {
+      m = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int i = 0; i < kDT; ++i) o[i] = Acc{};
+      KV::load(lds[0][0], k, a.k_row, 0, last, a.dim);
+      KV::load(lds[0][1], v, a.v_row, 0, last, a.dim);
+      all_tiles(Mode<2>());
+    }
   }
   l += swap_halves(l);
   store_row<VEC>(out, o, (DROP ? a.drop.scale : 1.f) / l, half, a.dim, inside);
@@ -362,7 +387,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_k(BfAttnArgs a) {
     QG::clear(&lds[0][0][0], sizeof(lds));
     __syncthreads();
   }
-  const auto fetch = [&](int h, int i0, int buf) {
+  const auto fetch = [&](int h, int i0, int buf) __attribute__((always_inline)) {
     const T* q = static_cast<const T*>(a.q) + static_cast<long>(w.begin) * a.q_row + h * a.q_head;
     const T* go = static_cast<const T*>(a.dout) + static_cast<long>(w.begin) * a.do_row + h * a.do_head;
     QG::load(lds[buf][0], q, a.q_row, i0, last, a.dim);

@@ -78,6 +78,7 @@ struct Tile {
   static constexpr int kChunks = DP / kEach;
   static constexpr int kRowBytes = DP * sizeof(T);
   static constexpr int kBytes = ROWS * kRowBytes;
+  static constexpr bool kFull = false;
 
   static __device__ __forceinline__ int swizzle(int r) {
     return kChunks == 8 ? (((r >> 1) & 3) << 1) | ((r >> 3) & 1) : ((r & 7) << 1) | ((r >> 3) & 1);
@@ -90,24 +91,27 @@ struct Tile {
   // register: a wave's load fills 1024 bytes, and each lane picks the chunk
   // that belongs there. Rows behind `last` repeat it (they are masked where
   // they would count, and hold nothing that their sequence does not). Columns
-  // behind dim stay as they are: cleared once.
+  // behind dim stay as they are: cleared once. A row is `stride` values wide,
+  // at most 2^22, so that places in a tile fit 32 bits.
   static __device__ __forceinline__ void load(char* lds, const T* base, long stride, int first, int last, int dim) {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const char* from = reinterpret_cast<const char*>(base + first * stride);
+    const uint32_t step = static_cast<uint32_t>(stride) * sizeof(T), most = (last - first) * step;
     if constexpr (VEC) {
 #pragma unroll
       for (int n = 0; n < kBytes / 1024 / (THREADS / 64); ++n) {
         const int block = n * (THREADS / 64) + wave;
         const int off = block * 1024 + lane * 16;
         const int row = off / kRowBytes, chunk = ((off % kRowBytes) >> 4) ^ swizzle(row);
-        const T* from = base + static_cast<long>(min(first + row, last)) * stride + chunk * kEach;
-        if (chunk * kEach < dim) load_to_lds<16>(from, lds + block * 1024);
+        const uint32_t at = min(row * step, most) + chunk * 16;
+        if (kFull || chunk * kEach < dim) load_to_lds<16>(from + at, lds + block * 1024);
       }
     } else {
       for (int i = threadIdx.x; i < ROWS * DP; i += THREADS) {
         const int row = i / DP, c = i % DP;
         if (c < dim)
           *reinterpret_cast<T*>(lds + at(row, c / kEach) + (c % kEach) * sizeof(T)) =
-              base[static_cast<long>(min(first + row, last)) * stride + c];
+              *reinterpret_cast<const T*>(from + min(row * step, most) + c * sizeof(T));
       }
     }
   }

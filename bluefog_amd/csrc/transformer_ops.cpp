@@ -80,12 +80,13 @@ bool any_grad(std::initializer_list<const Tensor*> ts) {
 // attention
 // ---------------------------------------------------------------------------
 
-// Whether rows and heads of t are dense along the last dimension and, where
-// a head fills whole 16-byte accesses, start on one. Other tensors are copied:
+// Whether rows and heads of t are dense along the last dimension, rows are
+// less than 2^22 values apart (a tile's places fit 32 bits) and, where a head
+// fills whole 16-byte accesses, start on one. Other tensors are copied:
 // a copy is cheaper than element-wise reads by every tile.
 Tensor readable(const Tensor& t) {
   const int64_t e = t.element_size(), d = t.size(2);
-  bool ok = t.stride(2) == 1 || d == 1;
+  bool ok = (t.stride(2) == 1 || d == 1) && (t.size(0) == 1 || t.stride(0) <= 1 << 22);
   if (d * e % 16 == 0) {
     ok = ok && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
     for (int i = 0; i < 2; ++i) ok = ok && (t.size(i) == 1 || t.stride(i) * e % 16 == 0);
