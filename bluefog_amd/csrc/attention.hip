@@ -350,19 +350,45 @@ __global__ __launch_bounds__(256, 2) void attn_dq_k(BfAttnArgs a) {
 // are the operands of dv^T = dO^T P and dk^T = q^T dS as they stand.
 // ---------------------------------------------------------------------------
 
+// A workgroup has 128 keys. Four waves have them, and where SPLIT is 2 four more
+// have them again and take the other half of each step's 64 queries; their sums
+// meet in LDS at the end. So one workgroup fills a CU, and a long sequence under
+// few key heads does not leave half a CU idle.
+template <typename T, int DP>
+constexpr int kSplit = sizeof(T) == 4 && DP == 128 ? 1 : 2;  // f32: LDS holds 32 queries a step
+
+// the sums of the second four waves to those of the first, through LDS
+template <int TILES>
+__device__ __forceinline__ void join(Acc (&acc)[TILES], void* lds, int part) {
+  Acc* place = static_cast<Acc*>(lds) + ((threadIdx.x >> 6) & 3) * TILES * 64 + (threadIdx.x & 63);
+  if (part) {
+#pragma unroll
+    for (int i = 0; i < TILES; ++i) place[i * 64] = acc[i];
+  }
+  __syncthreads();
+  if (!part) {
+#pragma unroll
+    for (int i = 0; i < TILES; ++i) acc[i] += place[i * 64];
+  }
+}
+
 template <typename T, int DP, bool VEC, bool DROP>
-__global__ __launch_bounds__(256, 2) void attn_dkv_k(BfAttnArgs a) {
-  constexpr int kK = 128, BM = kKeys<T>, kSub = BM / 32, kSteps = DP / 16, kDT = DP / 32;
-  typedef Tile<T, BM, DP, 256, VEC> QG;
+__global__ __launch_bounds__((256 * kSplit<T, DP>), 2) void attn_dkv_k(BfAttnArgs a) {
+  constexpr int kK = 128, SPLIT = kSplit<T, DP>, THREADS = 256 * SPLIT, BM = 32 * SPLIT;
+  constexpr int kSteps = DP / 16, kDT = DP / 32;
+  constexpr bool V_IN_LDS = DP == 128;  // registers hold the sums and k
+  typedef Tile<T, BM, DP, THREADS, VEC> QG;
+  typedef Tile<T, kK, DP, THREADS, VEC> Values;
   __shared__ __align__(1024) char lds[2][2][QG::kBytes];
-  __shared__ __align__(16) float stat[2][2][BM];       // lse and delta of the tile's queries
-  __shared__ __align__(16) uint32_t kept[4][DROP ? 32 : 4];  // a wave's mask: a query's 32 keys to a word
-  const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
+  __shared__ __align__(1024) char v_lds[V_IN_LDS ? Values::kBytes : 16];
+  __shared__ __align__(16) float stat[2][2][64];  // lse and delta of the tile's queries
+  __shared__ __align__(16) uint32_t kept[4 * SPLIT][DROP ? 32 : 4];  // a wave's mask: a query's 32 keys to a word
+  const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6, part = wave >> 2;
   const int g = blockIdx.x % a.kv_heads, group = a.heads / a.kv_heads;
   const Work w = find_tile(a, blockIdx.x / a.kv_heads, kK);
   if (!w.any) return;
-  const int j0 = w.tile * kK, jw = j0 + wave * 32, ji = jw + (lane & 31);
-  const bool inside = ji < w.len;
+  const int j0 = w.tile * kK, jl = (wave & 3) * 32 + (lane & 31), jw = j0 + (wave & 3) * 32, ji = j0 + jl;
+  const bool inside = ji < w.len && part == 0;
   const long row = w.begin + min(ji, w.len - 1), out = (row * a.kv_heads + g) * a.dim;
   Acc dk[kDT], dv[kDT];
 #pragma unroll
@@ -372,21 +398,25 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_k(BfAttnArgs a) {
     store_row<VEC>(static_cast<T*>(a.dv) + out, dv, 0.f, half, a.dim, inside);
     return;
   }
-  Frag<T> kf[kSteps], vf[kSteps];
+  const int last = w.len - 1;
+  if (a.dim < DP) {
+    QG::clear(&lds[0][0][0], sizeof(lds));
+    if (V_IN_LDS) Values::clear(v_lds, sizeof(v_lds));
+    __syncthreads();
+  }
+  Frag<T> kf[kSteps], vf[V_IN_LDS ? 1 : kSteps];
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
     kf[s] = load_row<VEC>(static_cast<const T*>(a.k) + row * a.k_row + g * a.k_head, s, half, a.dim);
-    vf[s] = load_row<VEC>(static_cast<const T*>(a.v) + row * a.v_row + g * a.v_head, s, half, a.dim);
+    if (!V_IN_LDS) vf[s] = load_row<VEC>(static_cast<const T*>(a.v) + row * a.v_row + g * a.v_head, s, half, a.dim);
   }
-  const int last = w.len - 1;
+  if (V_IN_LDS)
+    Values::load(v_lds, static_cast<const T*>(a.v) + static_cast<long>(w.begin) * a.v_row + g * a.v_head, a.v_row, j0, last,
+            a.dim);
   const int first = a.causal ? j0 / BM * BM : 0;  // queries in front of the keys see none of them
   const int from = a.causal ? ji : 0;  // first query that sees the lane's key
   const int from_ds = a.causal ? max(ji, 1) : w.len == 1 ? 1 : 0;  // and has another: with one key dS is 0
   const int total = (w.len - first + BM - 1) / BM * group;
-  if (a.dim < DP) {
-    QG::clear(&lds[0][0][0], sizeof(lds));
-    __syncthreads();
-  }
   const auto fetch = [&](int h, int i0, int buf) __attribute__((always_inline)) {
     const T* q = static_cast<const T*>(a.q) + static_cast<long>(w.begin) * a.q_row + h * a.q_head;
     const T* go = static_cast<const T*>(a.dout) + static_cast<long>(w.begin) * a.do_row + h * a.do_head;
@@ -407,80 +437,90 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_k(BfAttnArgs a) {
     next_h = h, next_i0 = i0 + BM;
     if (next_i0 >= w.len) ++next_h, next_i0 = first;
     if (n + 1 < total) fetch(next_h, next_i0, buf ^ 1);
-    if (jw < w.len && !(a.causal && i0 + BM - 1 < jw)) {
-      const bool masked = i0 + BM > w.len || (a.causal && (i0 < jw + 31 || i0 == 0)) || w.len == 1;
+    const int iw = i0 + part * 32;  // the wave's queries
+    if (jw < w.len && iw < w.len && !(a.causal && iw + 31 < jw)) {
+      const bool masked = iw + 32 > w.len || (a.causal && (iw < jw + 31 || iw == 0)) || w.len == 1;
+      Acc s{}, dp{};
 #pragma unroll
-      for (int u = 0; u < kSub; ++u) {
-        Acc s{}, dp{};
+      for (int i = 0; i < kSteps; ++i) s = mma(QG::read_row(lds[buf][0], part * 32 + (lane & 31), i, half), kf[i], s);
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) s = mma(QG::read_row(lds[buf][0], u * 32 + (lane & 31), i, half), kf[i], s);
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) dp = mma(QG::read_row(lds[buf][1], u * 32 + (lane & 31), i, half), vf[i], dp);
-        if (DROP) {
-          // the lane's share of a query's mask, as the forward pass has it
-          uint32_t bits = 0;
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const uint4 x = bf_philox((jw / 16 + t) * 2 + half, static_cast<uint32_t>(w.begin + i0 + u * 32 + (lane & 31)),
-                                      h, a.drop.offset, key);
-#pragma unroll
-            for (int r = 0; r < 8; ++r)
-              bits |= (bf_half(x, r) >= a.drop.threshold ? 1u : 0u) << (t * 16 + 8 * (r >> 2) + (r & 3));
-          }
-          bits <<= 4 * half;
-          bits |= __float_as_uint(swap_halves(__uint_as_float(bits)));
-          if (half == 0) kept[wave][lane] = bits;
-        }
-        float p[16], ds[16];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const float4 lse = *reinterpret_cast<const float4*>(&stat[buf][0][u * 32 + t * 8 + half * 4]);
-          const float4 delta = *reinterpret_cast<const float4*>(&stat[buf][1][u * 32 + t * 8 + half * 4]);
-          uint4 m = uint4{0, 0, 0, 0};
-          if (DROP) m = *reinterpret_cast<const uint4*>(&kept[wave][t * 8 + half * 4]);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float l = r == 0 ? lse.x : r == 1 ? lse.y : r == 2 ? lse.z : lse.w;
-            const float d = r == 0 ? delta.x : r == 1 ? delta.y : r == 2 ? delta.z : delta.w;
-            const uint32_t word = r == 0 ? m.x : r == 1 ? m.y : r == 2 ? m.z : m.w;
-            const float x = __builtin_amdgcn_exp2f(s[t * 4 + r] * c - (l - kPower<T>));
-            const bool keep = !DROP || (word >> (lane & 31)) & 1;
-            const float y = keep ? (DROP ? dp[t * 4 + r] * a.drop.scale : dp[t * 4 + r]) : 0.f;
-            p[t * 4 + r] = keep ? x : 0.f;
-            ds[t * 4 + r] = x * (y - d);
-          }
-        }
-        if (masked) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int i = i0 + u * 32 + row_of(r, half);
-            p[r] = i >= from && i < w.len ? p[r] : 0.f;
-            ds[r] = i >= from_ds && i < w.len ? ds[r] : 0.f;
-          }
-        }
-        if constexpr (kScaled<T>) {
-          rescale(dk, factor, ds);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) ds[r] *= factor;
-        }
+      for (int i = 0; i < kSteps; ++i)
+        dp = mma(QG::read_row(lds[buf][1], part * 32 + (lane & 31), i, half),
+                 V_IN_LDS ? Values::read_row(v_lds, jl, i, half) : vf[V_IN_LDS ? 0 : i], dp);
+      if (DROP) {
+        // the lane's share of a query's mask, as the forward pass has it
+        uint32_t bits = 0;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          Frag<T> pf, df;
+          const uint4 x = bf_philox((jw / 16 + t) * 2 + half, static_cast<uint32_t>(w.begin + iw + (lane & 31)), h,
+                                    a.drop.offset, key);
 #pragma unroll
-          for (int r = 0; r < 8; ++r) pf[r] = static_cast<T>(p[t * 8 + r]), df[r] = static_cast<T>(ds[t * 8 + r]);
+          for (int r = 0; r < 8; ++r)
+            bits |= (bf_half(x, r) >= a.drop.threshold ? 1u : 0u) << (t * 16 + 8 * (r >> 2) + (r & 3));
+        }
+        bits <<= 4 * half;
+        bits |= __float_as_uint(swap_halves(__uint_as_float(bits)));
+        if (half == 0) kept[wave][lane] = bits;
+      }
+      float p[16], ds[16];
 #pragma unroll
-          for (int i = 0; i < kDT; ++i) {
-            dv[i] = mma(QG::read_columns(lds[buf][1], u * 32 + t * 16, i, lane), pf, dv[i]);
-            dk[i] = mma(QG::read_columns(lds[buf][0], u * 32 + t * 16, i, lane), df, dk[i]);
-          }
+      for (int t = 0; t < 4; ++t) {
+        const float4 lse = *reinterpret_cast<const float4*>(&stat[buf][0][part * 32 + t * 8 + half * 4]);
+        const float4 delta = *reinterpret_cast<const float4*>(&stat[buf][1][part * 32 + t * 8 + half * 4]);
+        uint4 m = uint4{0, 0, 0, 0};
+        if (DROP) m = *reinterpret_cast<const uint4*>(&kept[wave][t * 8 + half * 4]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float l = r == 0 ? lse.x : r == 1 ? lse.y : r == 2 ? lse.z : lse.w;
+          const float d = r == 0 ? delta.x : r == 1 ? delta.y : r == 2 ? delta.z : delta.w;
+          const uint32_t word = r == 0 ? m.x : r == 1 ? m.y : r == 2 ? m.z : m.w;
+          const float x = __builtin_amdgcn_exp2f(s[t * 4 + r] * c - (l - kPower<T>));
+          const bool keep = !DROP || (word >> (lane & 31)) & 1;
+          const float y = keep ? (DROP ? dp[t * 4 + r] * a.drop.scale : dp[t * 4 + r]) : 0.f;
+          p[t * 4 + r] = keep ? x : 0.f;
+          ds[t * 4 + r] = x * (y - d);
+        }
+      }
+      if (masked) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int i = iw + row_of(r, half);
+          p[r] = i >= from && i < w.len ? p[r] : 0.f;
+          ds[r] = i >= from_ds && i < w.len ? ds[r] : 0.f;
+        }
+      }
+      if constexpr (kScaled<T>) {
+        rescale(dk, factor, ds);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) ds[r] *= factor;
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        Frag<T> pf, df;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) pf[r] = static_cast<T>(p[t * 8 + r]), df[r] = static_cast<T>(ds[t * 8 + r]);
+#pragma unroll
+        for (int i = 0; i < kDT; ++i) {
+          dv[i] = mma(QG::read_columns(lds[buf][1], part * 32 + t * 16, i, lane), pf, dv[i]);
+          dk[i] = mma(QG::read_columns(lds[buf][0], part * 32 + t * 16, i, lane), df, dk[i]);
         }
       }
     }
     loads_done();
   }
   const float power = exp2f(-kPower<T>), f = kScaled<T> ? (factor == 0.f ? 1.f : power / factor) : 1.f;
-  store_row<VEC>(static_cast<T*>(a.dk) + out, dk, a.scale * f, half, a.dim, inside);
-  store_row<VEC>(static_cast<T*>(a.dv) + out, dv, power * (DROP ? a.drop.scale : 1.f), half, a.dim, inside);
+#pragma unroll
+  for (int i = 0; i < kDT; ++i) {
+    dk[i] *= a.scale * f;
+    dv[i] *= power * (DROP ? a.drop.scale : 1.f);
+  }
+  if constexpr (SPLIT == 2) {
+    join(dk, &lds[0][0][0], part);
+    __syncthreads();
+    join(dv, &lds[0][0][0], part);
+  }
+  store_row<VEC>(static_cast<T*>(a.dk) + out, dk, 1.f, half, a.dim, inside);
+  store_row<VEC>(static_cast<T*>(a.dv) + out, dv, 1.f, half, a.dim, inside);
 }
 
 template <typename T, int DP, bool VEC>
@@ -504,7 +544,7 @@ hipError_t bwd(const BfAttnArgs& a, bool need_dkv, hipStream_t stream) {
   if (groups > 0x7FFFFFFF) return hipErrorInvalidValue;
   hipLaunchKernelGGL((attn_dq_k<T, DP, VEC, DROP>), dim3(groups), dim3(256), 0, stream, a);
   if (hipError_t e = hipGetLastError()) return e;
-  if (need_dkv) hipLaunchKernelGGL((attn_dkv_k<T, DP, VEC, DROP>), dim3(shared), dim3(256), 0, stream, a);
+  if (need_dkv) hipLaunchKernelGGL((attn_dkv_k<T, DP, VEC, DROP>), dim3(shared), dim3(256 * kSplit<T, DP>), 0, stream, a);
   return hipGetLastError();
 }
 
