@@ -61,16 +61,17 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_k(BfAttnArgs a) {
     return;
   }
   const T* q = static_cast<const T*>(a.q) + static_cast<long>(w.begin + min(qi, w.len - 1)) * a.q_row + h * a.q_head;
-  const T* k = static_cast<const T*>(a.k) + static_cast<long>(w.begin) * a.k_row + g * a.k_head;
-  const T* v = static_cast<const T*>(a.v) + static_cast<long>(w.begin) * a.v_row + g * a.v_head;
+  typedef Loader<T, BN, DP, 256, VEC> Load;
+  const Load k(static_cast<const T*>(a.k) + w.begin * a.k_row + g * a.k_head, a.k_row, a.dim);
+  const Load v(static_cast<const T*>(a.v) + w.begin * a.v_row + g * a.v_head, a.v_row, a.dim);
   const int last = w.len - 1, keys = a.causal ? min(w.len, q0 + kQ) : w.len;
   const int seen = a.causal ? min(w.len, qi + 1) : w.len;  // keys of the lane's row
   if (a.dim < DP) {
     KV::clear(&lds[0][0][0], sizeof(lds));
     __syncthreads();
   }
-  KV::load(lds[0][0], k, a.k_row, 0, last, a.dim);
-  KV::load(lds[0][1], v, a.v_row, 0, last, a.dim);
+  k.load(lds[0][0], 0, last);
+  v.load(lds[0][1], 0, last);
   Frag<T> qf[kSteps];
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) qf[s] = load_row<VEC>(q, s, half, a.dim);
@@ -158,8 +159,8 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_k(BfAttnArgs a) {
     int k0 = 0, buf = 0;
     const auto next = [&]() __attribute__((always_inline)) {
       if (k0 + BN >= keys) return;
-      KV::load(lds[buf ^ 1][0], k, a.k_row, k0 + BN, last, a.dim);
-      KV::load(lds[buf ^ 1][1], v, a.v_row, k0 + BN, last, a.dim);
+      k.load(lds[buf ^ 1][0], k0 + BN, last);
+      v.load(lds[buf ^ 1][1], k0 + BN, last);
     };
     for (; k0 < whole; k0 += BN, buf ^= 1) {
       next();
@@ -187,8 +188,8 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_k(BfAttnArgs a) {
       m = -INFINITY, l = 0.f;
 #pragma unroll
       for (int i = 0; i < kDT; ++i) o[i] = Acc{};
-      KV::load(lds[0][0], k, a.k_row, 0, last, a.dim);
-      KV::load(lds[0][1], v, a.v_row, 0, last, a.dim);
+      k.load(lds[0][0], 0, last);
+      v.load(lds[0][1], 0, last);
       all_tiles(Mode<2>());
     }
   }
@@ -254,15 +255,16 @@ __global__ __launch_bounds__(256, 2) void attn_dq_k(BfAttnArgs a) {
     store_row<VEC>(out, dq, 0.f, half, a.dim, inside);
     return;
   }
-  const T* k = static_cast<const T*>(a.k) + static_cast<long>(w.begin) * a.k_row + g * a.k_head;
-  const T* v = static_cast<const T*>(a.v) + static_cast<long>(w.begin) * a.v_row + g * a.v_head;
+  typedef Loader<T, BN, DP, 256, VEC> Load;
+  const Load k(static_cast<const T*>(a.k) + w.begin * a.k_row + g * a.k_head, a.k_row, a.dim);
+  const Load v(static_cast<const T*>(a.v) + w.begin * a.v_row + g * a.v_head, a.v_row, a.dim);
   const int last = w.len - 1, keys = a.causal ? min(w.len, q0 + kQ) : w.len;
   if (a.dim < DP) {
     KV::clear(&lds[0][0][0], sizeof(lds));
     __syncthreads();
   }
-  KV::load(lds[0][0], k, a.k_row, 0, last, a.dim);
-  KV::load(lds[0][1], v, a.v_row, 0, last, a.dim);
+  k.load(lds[0][0], 0, last);
+  v.load(lds[0][1], 0, last);
   Frag<T> qf[kSteps], gf[kSteps];
   float delta = 0.f;
   {
@@ -290,8 +292,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_k(BfAttnArgs a) {
   loads_done();
   for (int k0 = 0, buf = 0; k0 < keys; k0 += BN, buf ^= 1) {
     if (k0 + BN < keys) {
-      KV::load(lds[buf ^ 1][0], k, a.k_row, k0 + BN, last, a.dim);
-      KV::load(lds[buf ^ 1][1], v, a.v_row, k0 + BN, last, a.dim);
+      k.load(lds[buf ^ 1][0], k0 + BN, last);
+      v.load(lds[buf ^ 1][1], k0 + BN, last);
     }
     if (qw < w.len && !(a.causal && k0 > qw + 31)) {
       const bool masked = k0 + BN > w.len || (a.causal && (k0 + BN - 1 > qw || qw == 0));
@@ -411,17 +413,19 @@ __global__ __launch_bounds__((256 * kSplit<T, DP>), 2) void attn_dkv_k(BfAttnArg
     if (!V_IN_LDS) vf[s] = load_row<VEC>(static_cast<const T*>(a.v) + row * a.v_row + g * a.v_head, s, half, a.dim);
   }
   if (V_IN_LDS)
-    Values::load(v_lds, static_cast<const T*>(a.v) + static_cast<long>(w.begin) * a.v_row + g * a.v_head, a.v_row, j0, last,
-            a.dim);
+    Loader<T, kK, DP, THREADS, VEC>(static_cast<const T*>(a.v) + w.begin * a.v_row + g * a.v_head, a.v_row, a.dim)
+        .load(v_lds, j0, last);
   const int first = a.causal ? j0 / BM * BM : 0;  // queries in front of the keys see none of them
   const int from = a.causal ? ji : 0;  // first query that sees the lane's key
   const int from_ds = a.causal ? max(ji, 1) : w.len == 1 ? 1 : 0;  // and has another: with one key dS is 0
   const int total = (w.len - first + BM - 1) / BM * group;
+  typedef Loader<T, BM, DP, THREADS, VEC> Load;
+  Load q(nullptr, a.q_row, a.dim), go(nullptr, a.do_row, a.dim);
   const auto fetch = [&](int h, int i0, int buf) __attribute__((always_inline)) {
-    const T* q = static_cast<const T*>(a.q) + static_cast<long>(w.begin) * a.q_row + h * a.q_head;
-    const T* go = static_cast<const T*>(a.dout) + static_cast<long>(w.begin) * a.do_row + h * a.do_head;
-    QG::load(lds[buf][0], q, a.q_row, i0, last, a.dim);
-    QG::load(lds[buf][1], go, a.do_row, i0, last, a.dim);
+    q.base = reinterpret_cast<const char*>(static_cast<const T*>(a.q) + w.begin * a.q_row + h * a.q_head);
+    go.base = reinterpret_cast<const char*>(static_cast<const T*>(a.dout) + w.begin * a.do_row + h * a.do_head);
+    q.load(lds[buf][0], i0, last);
+    go.load(lds[buf][1], i0, last);
     if (wave < 2 && lane < BM) {
       const float* from = (wave ? a.delta : a.lse) + static_cast<long>(h) * a.rows + w.begin + min(i0 + lane, last);
       load_to_lds<4>(from, stat[buf][wave]);

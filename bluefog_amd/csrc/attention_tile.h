@@ -78,42 +78,12 @@ struct Tile {
   static constexpr int kChunks = DP / kEach;
   static constexpr int kRowBytes = DP * sizeof(T);
   static constexpr int kBytes = ROWS * kRowBytes;
-  static constexpr bool kFull = false;
 
   static __device__ __forceinline__ int swizzle(int r) {
     return kChunks == 8 ? (((r >> 1) & 3) << 1) | ((r >> 3) & 1) : ((r & 7) << 1) | ((r >> 3) & 1);
   }
   static __device__ __forceinline__ int at(int row, int chunk) {
     return row * kRowBytes + ((chunk ^ swizzle(row)) << 4);
-  }
-
-  // Rows first .. first + ROWS - 1 of a matrix into the tile, without a
-  // register: a wave's load fills 1024 bytes, and each lane picks the chunk
-  // that belongs there. Rows behind `last` repeat it (they are masked where
-  // they would count, and hold nothing that their sequence does not). Columns
-  // behind dim stay as they are: cleared once. A row is `stride` values wide,
-  // at most 2^22, so that places in a tile fit 32 bits.
-  static __device__ __forceinline__ void load(char* lds, const T* base, long stride, int first, int last, int dim) {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const char* from = reinterpret_cast<const char*>(base + first * stride);
-    const uint32_t step = static_cast<uint32_t>(stride) * sizeof(T), most = (last - first) * step;
-    if constexpr (VEC) {
-#pragma unroll
-      for (int n = 0; n < kBytes / 1024 / (THREADS / 64); ++n) {
-        const int block = n * (THREADS / 64) + wave;
-        const int off = block * 1024 + lane * 16;
-        const int row = off / kRowBytes, chunk = ((off % kRowBytes) >> 4) ^ swizzle(row);
-        const uint32_t at = min(row * step, most) + chunk * 16;
-        if (kFull || chunk * kEach < dim) load_to_lds<16>(from + at, lds + block * 1024);
-      }
-    } else {
-      for (int i = threadIdx.x; i < ROWS * DP; i += THREADS) {
-        const int row = i / DP, c = i % DP;
-        if (c < dim)
-          *reinterpret_cast<T*>(lds + at(row, c / kEach) + (c % kEach) * sizeof(T)) =
-              *reinterpret_cast<const T*>(from + min(row * step, most) + c * sizeof(T));
-      }
-    }
   }
 
   static __device__ __forceinline__ void clear(char* lds, int bytes) {
@@ -158,6 +128,66 @@ struct Tile {
         f[j] = *reinterpret_cast<const T*>(lds + at(base + row_of(j, half), c / kEach) + (c % kEach) * sizeof(T));
     }
     return f;
+  }
+};
+
+// Brings rows of a matrix into a tile, without a register: a wave's load fills
+// 1024 bytes, and each lane picks the chunk that belongs there. Rows behind
+// `last` repeat it (they are masked where they would count, and hold nothing
+// that their sequence does not). Columns behind dim stay as they are: cleared
+// once. A row is `stride` values wide, at most 2^22, so that places in a tile
+// fit 32 bits. All but one register of the addresses are scalar; worked out
+// load by load they were a third of the forward pass's vector instructions.
+template <typename T, int ROWS, int DP, int THREADS, bool VEC>
+struct Loader {
+  typedef Tile<T, ROWS, DP, THREADS, VEC> Of;
+  static constexpr int kLoads = Of::kBytes / (THREADS * 16);
+  static constexpr int kRound = THREADS * 16 / Of::kRowBytes;  // rows of the workgroup's loads number n
+  static constexpr bool kSame = kRound % 16 == 0;              // they have the same chunks for all n
+
+  const char* base;
+  uint32_t step;      // bytes of a row
+  int wave, dim;
+  uint32_t at;        // the lane's place in load 0
+  bool ok;            // its chunk has columns
+
+  __device__ __forceinline__ Loader(const T* first_row, long stride, int dim_)
+      : base(reinterpret_cast<const char*>(first_row)), step(static_cast<uint32_t>(stride) * sizeof(T)),
+        wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), dim(dim_) {
+    const uint32_t off = threadIdx.x * 16;
+    const int row = off / Of::kRowBytes, chunk = ((off % Of::kRowBytes) >> 4) ^ Of::swizzle(row);
+    at = row * step + chunk * 16;
+    ok = chunk * Of::kEach < dim;
+  }
+
+  __device__ __forceinline__ void load(char* lds, int first, int last) const {
+    const char* from = base + static_cast<uint64_t>(step) * static_cast<uint32_t>(first);
+    if constexpr (VEC) {
+      if (kSame && last - first >= ROWS - 1) {
+        if (ok)
+#pragma unroll
+          for (int n = 0; n < kLoads; ++n)
+            load_to_lds<16>(from + static_cast<uint64_t>(step) * (n * kRound) + at, lds + n * THREADS * 16 + wave * 1024);
+      } else {
+        const uint32_t most = (last - first) * step;
+        uint32_t off = threadIdx.x * 16;
+        asm volatile("" : "+v"(off));  // worked out here: kept over the loop, it would cost the loop registers
+#pragma unroll
+        for (int n = 0; n < kLoads; ++n) {
+          const int r = off / Of::kRowBytes + n * kRound, c = ((off % Of::kRowBytes) >> 4) ^ Of::swizzle(r);
+          if (c * Of::kEach < dim)
+            load_to_lds<16>(from + min(r * step, most) + c * 16, lds + n * THREADS * 16 + wave * 1024);
+        }
+      }
+    } else {
+      const uint32_t most = (last - first) * step;
+      for (uint32_t i = threadIdx.x; i < ROWS * DP; i += THREADS) {
+        const int r = i / DP, c = i % DP;
+        if (c < dim)
+          *reinterpret_cast<T*>(lds + Of::at(r, c / Of::kEach) + (c % Of::kEach) * sizeof(T)) =
+              *reinterpret_cast<const T*>(from + min(r * step, most) + c * sizeof(T));
+      }
+    }
   }
 };
 
