@@ -29,6 +29,10 @@ using namespace bf_attn;
 template <typename T>
 constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;  // keys of a tile
 
+// waves of a SIMD whose registers the kernels are held to
+template <typename T, int DP>
+constexpr int kWavesOf = sizeof(T) == 2 && DP == 64 ? 3 : 2;
+
 template <int N>
 struct Mode {
   static constexpr int value = N;
@@ -39,15 +43,15 @@ struct Mode {
 constexpr float kSlack = 8.f;
 
 template <typename T, int DP, bool VEC, bool DROP>
-__global__ __launch_bounds__(256, 2) void attn_fwd_k(BfAttnArgs a) {
+__global__ __launch_bounds__(256, (kWavesOf<T, DP>)) void attn_fwd_k(BfAttnArgs a) {
   constexpr int kQ = 128, BN = kKeys<T>, kSub = BN / 32, kSteps = DP / 16, kDT = DP / 32;
   typedef Tile<T, BN, DP, 256, VEC> KV;
   __shared__ __align__(1024) char lds[2][2][KV::kBytes];
   const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
-  const int h = blockIdx.x % a.heads, g = h / (a.heads / a.kv_heads);
-  Work w = find_tile(a, blockIdx.x / a.heads, kQ);
+  const Unit unit = unit_of(blockIdx.x, a.heads);
+  const int h = unit.head, g = h / (a.heads / a.kv_heads);
+  const Work w = find_tile(a, unit.number, kQ, a.causal);
   if (!w.any) return;
-  if (a.causal) w.tile = w.tiles - 1 - w.tile;  // the long ones first
   const int q0 = w.tile * kQ, qw = q0 + wave * 32, qi = qw + (lane & 31);
   const bool inside = qi < w.len;
   const long row = w.begin + qi;
@@ -235,15 +239,15 @@ __device__ __forceinline__ void rescale(Acc (&acc)[TILES], float& factor, const 
 }
 
 template <typename T, int DP, bool VEC, bool DROP>
-__global__ __launch_bounds__(256, 2) void attn_dq_k(BfAttnArgs a) {
+__global__ __launch_bounds__(256, (kWavesOf<T, DP>)) void attn_dq_k(BfAttnArgs a) {
   constexpr int kQ = 128, BN = kKeys<T>, kSub = BN / 32, kSteps = DP / 16, kDT = DP / 32;
   typedef Tile<T, BN, DP, 256, VEC> KV;
   __shared__ __align__(1024) char lds[2][2][KV::kBytes];
   const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
-  const int h = blockIdx.x % a.heads, g = h / (a.heads / a.kv_heads);
-  Work w = find_tile(a, blockIdx.x / a.heads, kQ);
+  const Unit unit = unit_of(blockIdx.x, a.heads);
+  const int h = unit.head, g = h / (a.heads / a.kv_heads);
+  const Work w = find_tile(a, unit.number, kQ, a.causal);
   if (!w.any) return;
-  if (a.causal) w.tile = w.tiles - 1 - w.tile;
   const int q0 = w.tile * kQ, qw = q0 + wave * 32, qi = qw + (lane & 31);
   const bool inside = qi < w.len;
   const long row = w.begin + min(qi, w.len - 1), at = static_cast<long>(h) * a.rows + row;
@@ -386,9 +390,11 @@ __global__ __launch_bounds__((256 * kSplit<T, DP>), 2) void attn_dkv_k(BfAttnArg
   __shared__ __align__(16) float stat[2][2][64];  // lse and delta of the tile's queries
   __shared__ __align__(16) uint32_t kept[4 * SPLIT][DROP ? 32 : 4];  // a wave's mask: a query's 32 keys to a word
   const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6, part = wave >> 2;
-  const int g = blockIdx.x % a.kv_heads, group = a.heads / a.kv_heads;
-  const Work w = find_tile(a, blockIdx.x / a.kv_heads, kK);
+  const Unit unit = unit_of(blockIdx.x, a.kv_heads);
+  const int g = unit.head, group = a.heads / a.kv_heads;
+  Work w = find_tile(a, unit.number, kK, a.causal);
   if (!w.any) return;
+  if (a.causal) w.tile = (w.len - 1) / kK - w.tile;  // the first keys have most queries
   const int j0 = w.tile * kK, jl = (wave & 3) * 32 + (lane & 31), jw = j0 + (wave & 3) * 32, ji = j0 + jl;
   const bool inside = ji < w.len && part == 0;
   const long row = w.begin + min(ji, w.len - 1), out = (row * a.kv_heads + g) * a.dim;
@@ -529,7 +535,7 @@ __global__ __launch_bounds__((256 * kSplit<T, DP>), 2) void attn_dkv_k(BfAttnArg
 
 template <typename T, int DP, bool VEC>
 hipError_t fwd(const BfAttnArgs& a, hipStream_t stream) {
-  const long groups = most_tiles(a, 128) * a.heads;
+  const long groups = units(most_tiles(a, 128), a.heads);
   if (groups > 0x7FFFFFFF) return hipErrorInvalidValue;
   if (a.drop.threshold) hipLaunchKernelGGL((attn_fwd_k<T, DP, VEC, true>), dim3(groups), dim3(256), 0, stream, a);
   else hipLaunchKernelGGL((attn_fwd_k<T, DP, VEC, false>), dim3(groups), dim3(256), 0, stream, a);
@@ -544,7 +550,7 @@ hipError_t fwd(const BfAttnArgs& a, hipStream_t stream) {
 
 template <typename T, int DP, bool VEC, bool DROP>
 hipError_t bwd(const BfAttnArgs& a, bool need_dkv, hipStream_t stream) {
-  const long groups = most_tiles(a, 128) * a.heads, shared = most_tiles(a, 128) * a.kv_heads;
+  const long groups = units(most_tiles(a, 128), a.heads), shared = units(most_tiles(a, 128), a.kv_heads);
   if (groups > 0x7FFFFFFF) return hipErrorInvalidValue;
   hipLaunchKernelGGL((attn_dq_k<T, DP, VEC, DROP>), dim3(groups), dim3(256), 0, stream, a);
   if (hipError_t e = hipGetLastError()) return e;

@@ -256,19 +256,40 @@ __device__ __forceinline__ float swap_halves(float x) {
 }
 
 // ---------------------------------------------------------------------------
-// Which rows a workgroup has. The sequences' tiles of `size` rows are numbered
-// through, and so are those of the rows behind the last sequence (`seq` ==
-// seqs then). Every wave searches by itself: lane i counts the tiles of
-// `chunk` sequences, the first lane whose running count exceeds the number has
-// it, and where chunk > 1 the same once more inside. Bounds that are not
-// ordered or leave [0, rows] are cut to it, so that no access leaves the
-// tensors.
+// Which rows a workgroup has.
+//
+// Workgroups go to the eight XCDs in turn, and each XCD has an L2 of its own. So
+// the heads are dealt out in runs, gcd(heads, 8) of them, and a run's tiles to
+// the XCDs that share it: what an XCD reads of k and v are few heads, and those
+// of a group together.
+//
+// The sequences' tiles of `size` rows are numbered through, and so are those
+// of the rows behind the last sequence (`seq` == seqs then). Bounds that are
+// not ordered or leave [0, rows] are cut to it, so that no access leaves the
+// tensors. Every wave searches by itself, a lane to a sequence.
 // ---------------------------------------------------------------------------
+
+struct Unit {
+  int head, number;
+};
+
+inline __host__ __device__ int runs_of(int heads) { return heads % 8 == 0 ? 8 : heads % 4 == 0 ? 4 : heads % 2 == 0 ? 2 : 1; }
+
+__device__ __forceinline__ Unit unit_of(int block, int heads) {
+  const int runs = runs_of(heads), each = heads / runs, share = 8 / runs;
+  const int xcd = block % 8, i = block / 8;
+  return {xcd % runs * each + i % each, i / each * share + xcd / runs};
+}
+
+// workgroups for `tiles` tiles of each head
+inline long units(long tiles, int heads) {
+  const int share = 8 / runs_of(heads);
+  return (tiles + share - 1) / share * share * heads;
+}
 
 struct Work {
   int begin, len;  // rows of the sequence
   int seq, tile;   // tile inside it
-  int tiles;       // of the sequence
   bool any;
 };
 
@@ -278,40 +299,69 @@ __device__ __forceinline__ int2 bounds_of(const BfAttnArgs& a, int seq) {
   return make_int2(begin, end);
 }
 
-__device__ __forceinline__ Work find_tile(const BfAttnArgs& a, int number, int size) {
+__device__ __forceinline__ int wave_sum(int x) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
+  return x;
+}
+
+__device__ __forceinline__ int sum_up_to(int x) {
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int y = __shfl_up(x, off, 64);
+    if ((threadIdx.x & 63) >= off) x += y;
+  }
+  return x;
+}
+
+// Tile `number`. Causal tiles cost the more the later they are (by_cost: the
+// later, from the sequence's end, the earlier), and a long one that starts last
+// keeps the card waiting: up to 63 sequences' tiles are numbered by their cost,
+// the most expensive first. More sequences, and tiles that cost the same inside
+// one, are numbered in order.
+__device__ __forceinline__ Work find_tile(const BfAttnArgs& a, int number, int size, bool by_cost) {
   const int lane = threadIdx.x & 63, n = a.seqs + 1;
   Work w{};
-  int first = 0, count = n, chunk = (n + 63) / 64;
-  while (true) {
-    int mine = 0;
-    for (int i = 0; i < chunk; ++i) {
-      const int s = first + lane * chunk + i;
-      if (lane * chunk + i < count) {
-        const int2 b = bounds_of(a, s);
-        mine += (b.y - b.x + size - 1) / size;
-      }
+  if (by_cost && n <= 64) {
+    const int2 b = lane < n ? bounds_of(a, lane) : make_int2(0, 0);
+    const int mine = (b.y - b.x + size - 1) / size;
+    int low = 0, high = a.rows / size + 1;  // more tiles than `number` cost `low` or more, and not `high`
+    if (wave_sum(mine) <= number) return w;
+    while (high - low > 1) {
+      const int mid = (low + high) / 2;
+      if (wave_sum(max(mine - mid, 0)) > number) low = mid;
+      else high = mid;
     }
-    int upto = mine;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int x = __shfl_up(upto, off, 64);
-      if (lane >= off) upto += x;
+    number -= wave_sum(max(mine - low - 1, 0));
+    const bool has = mine > low;
+    const unsigned long long past = __ballot(sum_up_to(has ? 1 : 0) > number);
+    w.seq = __ffsll(past) - 1;
+    w.tile = low;
+  } else {
+    int first = 0, count = n, chunk = (n + 63) / 64;
+    while (true) {
+      int mine = 0;
+      for (int i = 0; i < chunk; ++i)
+        if (lane * chunk + i < count) {
+          const int2 b = bounds_of(a, first + lane * chunk + i);
+          mine += (b.y - b.x + size - 1) / size;
+        }
+      const int upto = sum_up_to(mine);
+      const unsigned long long past = __ballot(upto > number);
+      if (!past) return w;
+      const int pick = __ffsll(past) - 1;
+      number -= __shfl(upto - mine, pick, 64);
+      first += pick * chunk;
+      if (chunk == 1) break;
+      count = min(chunk, count - pick * chunk);
+      chunk = (count + 63) / 64;
     }
-    const unsigned long long past = __ballot(upto > number);
-    if (!past) return w;
-    const int pick = __ffsll(past) - 1;
-    number -= __shfl(upto - mine, pick, 64);
-    first += pick * chunk;
-    if (chunk == 1) break;
-    count = min(chunk, count - pick * chunk);
-    chunk = (count + 63) / 64;
+    w.seq = __builtin_amdgcn_readfirstlane(first);
+    w.tile = __builtin_amdgcn_readfirstlane(number);
   }
-  w.seq = __builtin_amdgcn_readfirstlane(first);
-  w.tile = __builtin_amdgcn_readfirstlane(number);
   const int2 b = bounds_of(a, w.seq);
   w.begin = b.x;
   w.len = b.y - b.x;
-  w.tiles = (w.len + size - 1) / size;
   w.any = true;
   return w;
 }
