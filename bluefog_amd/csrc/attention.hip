@@ -14,6 +14,9 @@
 
 namespace {
 
+#ifndef BF_WANT
+#define BF_WANT 1024
+#endif
 constexpr float kLog2e = 1.4426950408889634f;
 
 using namespace bf_attn;
@@ -356,12 +359,30 @@ __global__ __launch_bounds__(256, (kWavesOf<T, DP>)) void attn_dq_k(BfAttnArgs a
 // are the operands of dv^T = dO^T P and dk^T = q^T dS as they stand.
 // ---------------------------------------------------------------------------
 
-// A workgroup has 128 keys. Four waves have them, and where SPLIT is 2 four more
-// have them again and take the other half of each step's 64 queries; their sums
-// meet in LDS at the end. So one workgroup fills a CU, and a long sequence under
-// few key heads does not leave half a CU idle.
+// A workgroup has 128 keys, four waves of 32, and a step is some queries of
+// one head. What a workgroup does in a step:
+//   SUBS  tiles of 32 queries that a wave takes
+//   SPLIT 2: four more waves have the same keys and take other queries; their
+//         sums meet in LDS at the end
+//   V_IN_LDS: v's fragments are read again rather than kept in registers
+//   WAVES of a SIMD whose registers it is held to
 template <typename T, int DP>
-constexpr int kSplit = sizeof(T) == 4 && DP == 128 ? 1 : 2;  // f32: LDS holds 32 queries a step
+struct DkvShape {
+  static constexpr int kSplit = 1, kSubs = sizeof(T) == 2 ? 2 : 1, kWaves = 2;
+  static constexpr bool kVInLds = false;
+};
+template <typename T>
+struct DkvShape<T, 128> {
+  static constexpr int kSplit = 2, kSubs = 1, kWaves = 2;
+  static constexpr bool kVInLds = true;
+};
+template <>
+struct DkvShape<float, 128> {  // LDS holds 32 queries a step
+  static constexpr int kSplit = 1, kSubs = 1, kWaves = 1;
+  static constexpr bool kVInLds = true;
+};
+template <typename T, int DP>
+constexpr int kDkvQueries = 32 * DkvShape<T, DP>::kSplit * DkvShape<T, DP>::kSubs;  // of a step
 
 // the sums of the second four waves to those of the first, through LDS
 template <int TILES>
@@ -379,10 +400,11 @@ __device__ __forceinline__ void join(Acc (&acc)[TILES], void* lds, int part) {
 }
 
 template <typename T, int DP, bool VEC, bool DROP>
-__global__ __launch_bounds__((256 * kSplit<T, DP>), 2) void attn_dkv_k(BfAttnArgs a) {
-  constexpr int kK = 128, SPLIT = kSplit<T, DP>, THREADS = 256 * SPLIT, BM = 32 * SPLIT;
+__global__ __launch_bounds__((256 * DkvShape<T, DP>::kSplit), (DkvShape<T, DP>::kWaves)) void attn_dkv_k(BfAttnArgs a) {
+  typedef DkvShape<T, DP> Shape;
+  constexpr int kK = 128, SPLIT = Shape::kSplit, SUBS = Shape::kSubs, THREADS = 256 * SPLIT, BM = kDkvQueries<T, DP>;
   constexpr int kSteps = DP / 16, kDT = DP / 32;
-  constexpr bool V_IN_LDS = DP == 128;  // registers hold the sums and k
+  constexpr bool V_IN_LDS = Shape::kVInLds;
   typedef Tile<T, BM, DP, THREADS, VEC> QG;
   typedef Tile<T, kK, DP, THREADS, VEC> Values;
   __shared__ __align__(1024) char lds[2][2][QG::kBytes];
@@ -392,7 +414,8 @@ __global__ __launch_bounds__((256 * kSplit<T, DP>), 2) void attn_dkv_k(BfAttnArg
   const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6, part = wave >> 2;
   const Unit unit = unit_of(blockIdx.x, a.kv_heads);
   const int g = unit.head, group = a.heads / a.kv_heads;
-  Work w = find_tile(a, unit.number, kK, a.causal);
+  const int slice = unit.number % a.slices;  // of the steps
+  Work w = find_tile(a, unit.number / a.slices, kK, a.causal);
   if (!w.any) return;
   if (a.causal) w.tile = (w.len - 1) / kK - w.tile;  // the first keys have most queries
   const int j0 = w.tile * kK, jl = (wave & 3) * 32 + (lane & 31), jw = j0 + (wave & 3) * 32, ji = j0 + jl;
@@ -401,9 +424,18 @@ __global__ __launch_bounds__((256 * kSplit<T, DP>), 2) void attn_dkv_k(BfAttnArg
   Acc dk[kDT], dv[kDT];
 #pragma unroll
   for (int i = 0; i < kDT; ++i) dk[i] = dv[i] = Acc{};
+  const auto finish = [&]() __attribute__((always_inline)) {
+    if (a.slices == 1) {
+      store_row<VEC>(static_cast<T*>(a.dk) + out, dk, 1.f, half, a.dim, inside);
+      store_row<VEC>(static_cast<T*>(a.dv) + out, dv, 1.f, half, a.dim, inside);
+    } else {
+      const long all = static_cast<long>(a.rows) * a.kv_heads * a.dim;
+      store_row<VEC>(a.partial + 2 * slice * all + out, dk, 1.f, half, a.dim, inside);
+      store_row<VEC>(a.partial + (2 * slice + 1) * all + out, dv, 1.f, half, a.dim, inside);
+    }
+  };
   if (w.seq == a.seqs) {  // behind the last sequence
-    store_row<VEC>(static_cast<T*>(a.dk) + out, dk, 0.f, half, a.dim, inside);
-    store_row<VEC>(static_cast<T*>(a.dv) + out, dv, 0.f, half, a.dim, inside);
+    finish();
     return;
   }
   const int last = w.len - 1;
@@ -424,7 +456,9 @@ __global__ __launch_bounds__((256 * kSplit<T, DP>), 2) void attn_dkv_k(BfAttnArg
   const int first = a.causal ? j0 / BM * BM : 0;  // queries in front of the keys see none of them
   const int from = a.causal ? ji : 0;  // first query that sees the lane's key
   const int from_ds = a.causal ? max(ji, 1) : w.len == 1 ? 1 : 0;  // and has another: with one key dS is 0
-  const int total = (w.len - first + BM - 1) / BM * group;
+  const int steps = (w.len - first + BM - 1) / BM, total = steps * group;
+  const int begin = static_cast<int>(static_cast<long>(total) * slice / a.slices);
+  const int end = static_cast<int>(static_cast<long>(total) * (slice + 1) / a.slices);
   typedef Loader<T, BM, DP, THREADS, VEC> Load;
   Load q(nullptr, a.q_row, a.dim), go(nullptr, a.do_row, a.dim);
   const auto fetch = [&](int h, int i0, int buf) __attribute__((always_inline)) {
@@ -440,79 +474,82 @@ __global__ __launch_bounds__((256 * kSplit<T, DP>), 2) void attn_dkv_k(BfAttnArg
   const BfKey key = DROP ? bf_key(a.drop) : BfKey{0, 0};
   const float c = a.scale * kLog2e;
   float factor = 0.f;
-  int h = g * group, i0 = first;  // head and queries of a step, and of the next
-  fetch(h, i0, 0);
+  int h = g * group + begin / steps, i0 = first + begin % steps * BM;  // head and queries of a step, and of the next
+  if (begin < end) fetch(h, i0, 0);
   loads_done();
-  for (int n = 0, buf = 0, next_h, next_i0; n < total; ++n, buf ^= 1, h = next_h, i0 = next_i0) {
+  for (int n = begin, buf = 0, next_h, next_i0; n < end; ++n, buf ^= 1, h = next_h, i0 = next_i0) {
     next_h = h, next_i0 = i0 + BM;
     if (next_i0 >= w.len) ++next_h, next_i0 = first;
-    if (n + 1 < total) fetch(next_h, next_i0, buf ^ 1);
-    const int iw = i0 + part * 32;  // the wave's queries
-    if (jw < w.len && iw < w.len && !(a.causal && iw + 31 < jw)) {
-      const bool masked = iw + 32 > w.len || (a.causal && (iw < jw + 31 || iw == 0)) || w.len == 1;
-      Acc s{}, dp{};
+    if (n + 1 < end) fetch(next_h, next_i0, buf ^ 1);
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) s = mma(QG::read_row(lds[buf][0], part * 32 + (lane & 31), i, half), kf[i], s);
+    for (int n32 = 0; n32 < SUBS; ++n32) {
+      const int sub = (part * SUBS + n32) * 32, iw = i0 + sub;  // the wave's queries
+      if (jw < w.len && iw < w.len && !(a.causal && iw + 31 < jw)) {
+        const bool masked = iw + 32 > w.len || (a.causal && (iw < jw + 31 || iw == 0)) || w.len == 1;
+        Acc s{}, dp{};
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i)
-        dp = mma(QG::read_row(lds[buf][1], part * 32 + (lane & 31), i, half),
-                 V_IN_LDS ? Values::read_row(v_lds, jl, i, half) : vf[V_IN_LDS ? 0 : i], dp);
-      if (DROP) {
-        // the lane's share of a query's mask, as the forward pass has it
-        uint32_t bits = 0;
+        for (int i = 0; i < kSteps; ++i) s = mma(QG::read_row(lds[buf][0], sub + (lane & 31), i, half), kf[i], s);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+          dp = mma(QG::read_row(lds[buf][1], sub + (lane & 31), i, half),
+                   V_IN_LDS ? Values::read_row(v_lds, jl, i, half) : vf[V_IN_LDS ? 0 : i], dp);
+        if (DROP) {
+          // the lane's share of a query's mask, as the forward pass has it
+          uint32_t bits = 0;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const uint4 x = bf_philox((jw / 16 + t) * 2 + half, static_cast<uint32_t>(w.begin + iw + (lane & 31)), h,
+                                      a.drop.offset, key);
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+              bits |= (bf_half(x, r) >= a.drop.threshold ? 1u : 0u) << (t * 16 + 8 * (r >> 2) + (r & 3));
+          }
+          bits <<= 4 * half;
+          bits |= __float_as_uint(swap_halves(__uint_as_float(bits)));
+          if (half == 0) kept[wave][lane] = bits;
+        }
+        float p[16], ds[16];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const float4 lse = *reinterpret_cast<const float4*>(&stat[buf][0][sub + t * 8 + half * 4]);
+          const float4 delta = *reinterpret_cast<const float4*>(&stat[buf][1][sub + t * 8 + half * 4]);
+          uint4 m = uint4{0, 0, 0, 0};
+          if (DROP) m = *reinterpret_cast<const uint4*>(&kept[wave][t * 8 + half * 4]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float l = r == 0 ? lse.x : r == 1 ? lse.y : r == 2 ? lse.z : lse.w;
+            const float d = r == 0 ? delta.x : r == 1 ? delta.y : r == 2 ? delta.z : delta.w;
+            const uint32_t word = r == 0 ? m.x : r == 1 ? m.y : r == 2 ? m.z : m.w;
+            const float x = __builtin_amdgcn_exp2f(s[t * 4 + r] * c - (l - kPower<T>));
+            const bool keep = !DROP || (word >> (lane & 31)) & 1;
+            const float y = keep ? (DROP ? dp[t * 4 + r] * a.drop.scale : dp[t * 4 + r]) : 0.f;
+            p[t * 4 + r] = keep ? x : 0.f;
+            ds[t * 4 + r] = x * (y - d);
+          }
+        }
+        if (masked) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int i = iw + row_of(r, half);
+            p[r] = i >= from && i < w.len ? p[r] : 0.f;
+            ds[r] = i >= from_ds && i < w.len ? ds[r] : 0.f;
+          }
+        }
+        if constexpr (kScaled<T>) {
+          rescale(dk, factor, ds);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) ds[r] *= factor;
+        }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const uint4 x = bf_philox((jw / 16 + t) * 2 + half, static_cast<uint32_t>(w.begin + iw + (lane & 31)), h,
-                                    a.drop.offset, key);
+          Frag<T> pf, df;
 #pragma unroll
-          for (int r = 0; r < 8; ++r)
-            bits |= (bf_half(x, r) >= a.drop.threshold ? 1u : 0u) << (t * 16 + 8 * (r >> 2) + (r & 3));
-        }
-        bits <<= 4 * half;
-        bits |= __float_as_uint(swap_halves(__uint_as_float(bits)));
-        if (half == 0) kept[wave][lane] = bits;
-      }
-      float p[16], ds[16];
+          for (int r = 0; r < 8; ++r) pf[r] = static_cast<T>(p[t * 8 + r]), df[r] = static_cast<T>(ds[t * 8 + r]);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const float4 lse = *reinterpret_cast<const float4*>(&stat[buf][0][part * 32 + t * 8 + half * 4]);
-        const float4 delta = *reinterpret_cast<const float4*>(&stat[buf][1][part * 32 + t * 8 + half * 4]);
-        uint4 m = uint4{0, 0, 0, 0};
-        if (DROP) m = *reinterpret_cast<const uint4*>(&kept[wave][t * 8 + half * 4]);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float l = r == 0 ? lse.x : r == 1 ? lse.y : r == 2 ? lse.z : lse.w;
-          const float d = r == 0 ? delta.x : r == 1 ? delta.y : r == 2 ? delta.z : delta.w;
-          const uint32_t word = r == 0 ? m.x : r == 1 ? m.y : r == 2 ? m.z : m.w;
-          const float x = __builtin_amdgcn_exp2f(s[t * 4 + r] * c - (l - kPower<T>));
-          const bool keep = !DROP || (word >> (lane & 31)) & 1;
-          const float y = keep ? (DROP ? dp[t * 4 + r] * a.drop.scale : dp[t * 4 + r]) : 0.f;
-          p[t * 4 + r] = keep ? x : 0.f;
-          ds[t * 4 + r] = x * (y - d);
-        }
-      }
-      if (masked) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int i = iw + row_of(r, half);
-          p[r] = i >= from && i < w.len ? p[r] : 0.f;
-          ds[r] = i >= from_ds && i < w.len ? ds[r] : 0.f;
-        }
-      }
-      if constexpr (kScaled<T>) {
-        rescale(dk, factor, ds);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) ds[r] *= factor;
-      }
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        Frag<T> pf, df;
-#pragma unroll
-        for (int r = 0; r < 8; ++r) pf[r] = static_cast<T>(p[t * 8 + r]), df[r] = static_cast<T>(ds[t * 8 + r]);
-#pragma unroll
-        for (int i = 0; i < kDT; ++i) {
-          dv[i] = mma(QG::read_columns(lds[buf][1], part * 32 + t * 16, i, lane), pf, dv[i]);
-          dk[i] = mma(QG::read_columns(lds[buf][0], part * 32 + t * 16, i, lane), df, dk[i]);
+          for (int i = 0; i < kDT; ++i) {
+            dv[i] = mma(QG::read_columns(lds[buf][1], sub + t * 16, i, lane), pf, dv[i]);
+            dk[i] = mma(QG::read_columns(lds[buf][0], sub + t * 16, i, lane), df, dk[i]);
+          }
         }
       }
     }
@@ -529,8 +566,24 @@ __global__ __launch_bounds__((256 * kSplit<T, DP>), 2) void attn_dkv_k(BfAttnArg
     __syncthreads();
     join(dv, &lds[0][0][0], part);
   }
-  store_row<VEC>(static_cast<T*>(a.dk) + out, dk, 1.f, half, a.dim, inside);
-  store_row<VEC>(static_cast<T*>(a.dv) + out, dv, 1.f, half, a.dim, inside);
+  finish();
+}
+
+// the slices' dk and dv, one behind the other, in a fixed order
+template <typename T>
+__global__ __launch_bounds__(256) void attn_fold_k(T* dk, T* dv, const float* partial, long all, int slices) {
+  const long i = (static_cast<long>(blockIdx.x) * 256 + threadIdx.x) * 4;
+  if (i >= all) return;
+  const int n = all - i < 4 ? static_cast<int>(all - i) : 4;
+  partial += blockIdx.y * all + i;
+  float sum[4] = {};
+  for (int s = 0; s < slices; ++s)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) sum[u] += u < n ? partial[2 * s * all + u] : 0.f;
+  T* out = (blockIdx.y ? dv : dk) + i;
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (u < n) out[u] = static_cast<T>(sum[u]);
 }
 
 template <typename T, int DP, bool VEC>
@@ -550,11 +603,18 @@ hipError_t fwd(const BfAttnArgs& a, hipStream_t stream) {
 
 template <typename T, int DP, bool VEC, bool DROP>
 hipError_t bwd(const BfAttnArgs& a, bool need_dkv, hipStream_t stream) {
-  const long groups = units(most_tiles(a, 128), a.heads), shared = units(most_tiles(a, 128), a.kv_heads);
-  if (groups > 0x7FFFFFFF) return hipErrorInvalidValue;
+  const long groups = units(most_tiles(a, 128), a.heads), shared = units(most_tiles(a, 128) * a.slices, a.kv_heads);
+  if (groups > 0x7FFFFFFF || shared > 0x7FFFFFFF) return hipErrorInvalidValue;
   hipLaunchKernelGGL((attn_dq_k<T, DP, VEC, DROP>), dim3(groups), dim3(256), 0, stream, a);
   if (hipError_t e = hipGetLastError()) return e;
-  if (need_dkv) hipLaunchKernelGGL((attn_dkv_k<T, DP, VEC, DROP>), dim3(shared), dim3(256 * kSplit<T, DP>), 0, stream, a);
+  if (!need_dkv) return hipSuccess;
+  hipLaunchKernelGGL((attn_dkv_k<T, DP, VEC, DROP>), dim3(shared), dim3(256 * DkvShape<T, DP>::kSplit), 0, stream, a);
+  if (hipError_t e = hipGetLastError()) return e;
+  if (a.slices == 1) return hipSuccess;
+  const long all = static_cast<long>(a.rows) * a.kv_heads * a.dim, blocks = (all + 1023) / 1024;
+  if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(attn_fold_k<T>, dim3(blocks, 2), dim3(256), 0, stream, static_cast<T*>(a.dk), static_cast<T*>(a.dv),
+                     a.partial, all, a.slices);
   return hipGetLastError();
 }
 
@@ -572,6 +632,18 @@ hipError_t bwd(const BfAttnArgs& a, bool need_dkv, hipStream_t stream) {
 }  // namespace
 
 extern "C" {
+
+// Slices of the queries in the dk and dv pass. A workgroup goes over all queries
+// of a head group, so few key heads or long sequences leave few workgroups; each
+// slice more costs 16 bytes of memory traffic for a value of dk and dv.
+int bf_attn_slices(const BfAttnArgs* a) {
+  const long groups = (a->rows + 127L) / 128 * a->kv_heads;
+  const long length = a->rows / (a->seqs > 0 ? a->seqs : 1);
+  const long steps = (length + 63) / 64 * (a->heads / a->kv_heads);
+  const long wanted = (BF_WANT + groups - 1) / groups, most = steps / 4;
+  const long n = wanted < most ? wanted : most;
+  return static_cast<int>(n < 1 ? 1 : n > 16 ? 16 : n);
+}
 
 hipError_t bf_attn_fwd(const BfAttnArgs* a, int dtype, hipStream_t stream) {
   switch (dtype) {

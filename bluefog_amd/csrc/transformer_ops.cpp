@@ -173,6 +173,12 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
       a.dq = dq.data_ptr();
       a.dk = dk.data_ptr();
       a.dv = dv.data_ptr();
+      a.slices = bf_attn_slices(&a);
+      Tensor partial;
+      if (a.slices > 1 && need_dkv) {
+        partial = at::empty({a.slices, 2, dk.numel()}, lse.options());
+        a.partial = partial.data_ptr<float>();
+      }
       check(bf_attn_bwd(&a, code_of(q), need_dq, need_dkv, stream_of(q)), "packed_attention backward");
     }
     none[0] = dq, none[1] = dk, none[2] = dv;
