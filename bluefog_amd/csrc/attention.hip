@@ -16,6 +16,7 @@ namespace {
 
 #ifndef BF_WANT
 #define BF_WANT 1024
+#define BF_WANTQ 768
 #endif
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -36,6 +37,12 @@ constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;  // keys of a tile
 template <typename T, int DP>
 constexpr int kWavesOf = sizeof(T) == 2 && DP == 64 ? 3 : 2;
 
+// a slice's keys of `keys`, whole tiles
+__device__ __forceinline__ int2 keys_of(int keys, int tile, int slice, int slices) {
+  const int tiles = (keys + tile - 1) / tile;
+  return make_int2(tiles * slice / slices * tile, min(keys, tiles * (slice + 1) / slices * tile));
+}
+
 template <int N>
 struct Mode {
   static constexpr int value = N;
@@ -53,32 +60,48 @@ __global__ __launch_bounds__(256, (kWavesOf<T, DP>)) void attn_fwd_k(BfAttnArgs 
   const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
   const Unit unit = unit_of(blockIdx.x, a.heads);
   const int h = unit.head, g = h / (a.heads / a.kv_heads);
-  const Work w = find_tile(a, unit.number, kQ, a.causal);
+  const int slice = unit.number % a.key_slices;  // of the keys
+  const Work w = find_tile(a, unit.number / a.key_slices, kQ, a.causal);
   if (!w.any) return;
   const int q0 = w.tile * kQ, qw = q0 + wave * 32, qi = qw + (lane & 31);
   const bool inside = qi < w.len;
   const long row = w.begin + qi;
-  T* out = static_cast<T*>(a.o) + (row * a.heads + h) * a.dim;
   Acc o[kDT];
 #pragma unroll
   for (int i = 0; i < kDT; ++i) o[i] = Acc{};
+  // o times f, and the logarithm of its sum to base 2
+  const auto finish = [&](float f, float lse) __attribute__((always_inline)) {
+    const long at = (row * a.heads + h) * a.dim, all = static_cast<long>(a.rows) * a.heads;
+    if (a.key_slices == 1) {
+      store_row<VEC>(static_cast<T*>(a.o) + at, o, f, half, a.dim, inside);
+      if (a.lse && inside && half == 0) a.lse[static_cast<long>(h) * a.rows + row] = lse;
+    } else {
+      store_row<VEC>(a.partial + slice * all * a.dim + at, o, f, half, a.dim, inside);
+      float* sums = a.partial + a.key_slices * all * a.dim;
+      if (inside && half == 0) sums[slice * all + static_cast<long>(h) * a.rows + row] = lse;
+    }
+  };
   if (w.seq == a.seqs) {  // behind the last sequence
-    store_row<VEC>(out, o, 0.f, half, a.dim, inside);
-    if (a.lse && inside && half == 0) a.lse[static_cast<long>(h) * a.rows + row] = 0.f;
+    finish(0.f, 0.f);
     return;
   }
   const T* q = static_cast<const T*>(a.q) + static_cast<long>(w.begin + min(qi, w.len - 1)) * a.q_row + h * a.q_head;
   typedef Loader<T, BN, DP, 256, VEC> Load;
   const Load k(static_cast<const T*>(a.k) + w.begin * a.k_row + g * a.k_head, a.k_row, a.dim);
   const Load v(static_cast<const T*>(a.v) + w.begin * a.v_row + g * a.v_head, a.v_row, a.dim);
-  const int last = w.len - 1, keys = a.causal ? min(w.len, q0 + kQ) : w.len;
+  const int last = w.len - 1;
   const int seen = a.causal ? min(w.len, qi + 1) : w.len;  // keys of the lane's row
+  const int2 range = keys_of(a.causal ? min(w.len, q0 + kQ) : w.len, BN, slice, a.key_slices);
+  if (range.x >= range.y) {
+    finish(0.f, -INFINITY);
+    return;
+  }
   if (a.dim < DP) {
     KV::clear(&lds[0][0][0], sizeof(lds));
     __syncthreads();
   }
-  k.load(lds[0][0], 0, last);
-  v.load(lds[0][1], 0, last);
+  k.load(lds[0][0], range.x, last);
+  v.load(lds[0][1], range.x, last);
   Frag<T> qf[kSteps];
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) qf[s] = load_row<VEC>(q, s, half, a.dim);
@@ -161,11 +184,11 @@ __global__ __launch_bounds__(256, (kWavesOf<T, DP>)) void attn_fwd_k(BfAttnArgs 
   // all tiles, from the one whose load is under way into buffer 0; those that
   // no row has to mask have a loop of their own
   const auto all_tiles = [&](auto masked) __attribute__((always_inline)) {
-    const int whole = a.causal ? (q0 + 1) / BN * BN : w.len / BN * BN;
+    const int whole = min(range.y, (a.causal ? q0 + 1 : w.len) / BN * BN);
     loads_done();
-    int k0 = 0, buf = 0;
+    int k0 = range.x, buf = 0;
     const auto next = [&]() __attribute__((always_inline)) {
-      if (k0 + BN >= keys) return;
+      if (k0 + BN >= range.y) return;
       k.load(lds[buf ^ 1][0], k0 + BN, last);
       v.load(lds[buf ^ 1][1], k0 + BN, last);
     };
@@ -174,7 +197,7 @@ __global__ __launch_bounds__(256, (kWavesOf<T, DP>)) void attn_fwd_k(BfAttnArgs 
       if (qw < w.len) attend(Mode<0>(), k0, buf);
       loads_done();
     }
-    for (; k0 < keys; k0 += BN, buf ^= 1) {
+    for (; k0 < range.y; k0 += BN, buf ^= 1) {
       next();
       if (qw < w.len && !(a.causal && k0 > qw + 31)) attend(masked, k0, buf);
       loads_done();
@@ -195,14 +218,42 @@ __global__ __launch_bounds__(256, (kWavesOf<T, DP>)) void attn_fwd_k(BfAttnArgs 
       m = -INFINITY, l = 0.f;
 #pragma unroll
       for (int i = 0; i < kDT; ++i) o[i] = Acc{};
-      k.load(lds[0][0], 0, last);
-      v.load(lds[0][1], 0, last);
+      k.load(lds[0][0], range.x, last);
+      v.load(lds[0][1], range.x, last);
       all_tiles(Mode<2>());
     }
   }
   l += swap_halves(l);
-  store_row<VEC>(out, o, (DROP ? a.drop.scale : 1.f) / l, half, a.dim, inside);
-  if (a.lse && inside && half == 0) a.lse[static_cast<long>(h) * a.rows + row] = m * c + log2f(l);
+  // a slice may have no key that the row sees; a row whose scores are all -inf
+  // has no softmax
+  const bool none = a.key_slices > 1 && l == 0.f;
+  finish(none ? 0.f : (DROP ? a.drop.scale : 1.f) / l, none ? -INFINITY : m * c + log2f(l));
+}
+
+// the slices' rows into one, each by its share of the sum: four columns a lane
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join_k(BfAttnArgs a) {
+  const long all = static_cast<long>(a.rows) * a.heads;
+  const int each = (a.dim + 3) / 4;
+  const long i = static_cast<long>(blockIdx.x) * 256 + threadIdx.x;
+  const long at = i / each;  // row and head
+  const int c = static_cast<int>(i % each) * 4, n = min(4, a.dim - c);
+  if (at >= all) return;
+  const float* sums = a.partial + a.key_slices * all * a.dim + at % a.heads * a.rows + at / a.heads;
+  float top = -INFINITY, total = 0.f, out[4] = {};
+  for (int s = 0; s < a.key_slices; ++s) top = fmaxf(top, sums[s * all]);
+  for (int s = 0; s < a.key_slices; ++s) {
+    const float share = exp2f(sums[s * all] - top);
+    const float* part = a.partial + (s * all + at) * a.dim + c;
+    total += share;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) out[u] += u < n ? share * part[u] : 0.f;
+  }
+  T* o = static_cast<T*>(a.o) + at * a.dim + c;
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (u < n) o[u] = static_cast<T>(out[u] / total);
+  if (a.lse && c == 0) a.lse[at % a.heads * a.rows + at / a.heads] = top + log2f(total);
 }
 
 // ---------------------------------------------------------------------------
@@ -249,29 +300,40 @@ __global__ __launch_bounds__(256, (kWavesOf<T, DP>)) void attn_dq_k(BfAttnArgs a
   const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
   const Unit unit = unit_of(blockIdx.x, a.heads);
   const int h = unit.head, g = h / (a.heads / a.kv_heads);
-  const Work w = find_tile(a, unit.number, kQ, a.causal);
+  const int slice = unit.number % a.key_slices;
+  const Work w = find_tile(a, unit.number / a.key_slices, kQ, a.causal);
   if (!w.any) return;
   const int q0 = w.tile * kQ, qw = q0 + wave * 32, qi = qw + (lane & 31);
   const bool inside = qi < w.len;
   const long row = w.begin + min(qi, w.len - 1), at = static_cast<long>(h) * a.rows + row;
-  T* out = static_cast<T*>(a.dq) + (row * a.heads + h) * a.dim;
   Acc dq[kDT];
 #pragma unroll
   for (int i = 0; i < kDT; ++i) dq[i] = Acc{};
+  const auto finish = [&](float f) __attribute__((always_inline)) {
+    const long out = (row * a.heads + h) * a.dim;
+    if (a.key_slices == 1) store_row<VEC>(static_cast<T*>(a.dq) + out, dq, f, half, a.dim, inside);
+    else
+      store_row<VEC>(a.partial + slice * static_cast<long>(a.rows) * a.heads * a.dim + out, dq, f, half, a.dim, inside);
+  };
   if (w.seq == a.seqs) {  // behind the last sequence
-    store_row<VEC>(out, dq, 0.f, half, a.dim, inside);
+    finish(0.f);
     return;
   }
   typedef Loader<T, BN, DP, 256, VEC> Load;
   const Load k(static_cast<const T*>(a.k) + w.begin * a.k_row + g * a.k_head, a.k_row, a.dim);
   const Load v(static_cast<const T*>(a.v) + w.begin * a.v_row + g * a.v_head, a.v_row, a.dim);
-  const int last = w.len - 1, keys = a.causal ? min(w.len, q0 + kQ) : w.len;
+  const int last = w.len - 1;
+  const int2 range = keys_of(a.causal ? min(w.len, q0 + kQ) : w.len, BN, slice, a.key_slices);
+  if (range.x >= range.y && slice) {  // slice 0 has delta to write
+    finish(0.f);
+    return;
+  }
   if (a.dim < DP) {
     KV::clear(&lds[0][0][0], sizeof(lds));
     __syncthreads();
   }
-  k.load(lds[0][0], 0, last);
-  v.load(lds[0][1], 0, last);
+  k.load(lds[0][0], range.x, last);
+  v.load(lds[0][1], range.x, last);
   Frag<T> qf[kSteps], gf[kSteps];
   float delta = 0.f;
   {
@@ -288,7 +350,7 @@ __global__ __launch_bounds__(256, (kWavesOf<T, DP>)) void attn_dq_k(BfAttnArgs a
     }
     delta += swap_halves(delta);
   }
-  if (inside && half == 0) a.delta[at] = delta;
+  if (inside && half == 0 && slice == 0) a.delta[at] = delta;
   const BfKey key = DROP ? bf_key(a.drop) : BfKey{0, 0};
   const float c = a.scale * kLog2e, lse = a.lse[at] - kPower<T>;
   // keys of the lane's row that have a dS: a row that sees one key has P = 1
@@ -297,8 +359,8 @@ __global__ __launch_bounds__(256, (kWavesOf<T, DP>)) void attn_dq_k(BfAttnArgs a
   seen = seen == 1 ? 0 : seen;
   float factor = 0.f;  // f16: what dS is held times
   loads_done();
-  for (int k0 = 0, buf = 0; k0 < keys; k0 += BN, buf ^= 1) {
-    if (k0 + BN < keys) {
+  for (int k0 = range.x, buf = 0; k0 < range.y; k0 += BN, buf ^= 1) {
+    if (k0 + BN < range.y) {
       k.load(lds[buf ^ 1][0], k0 + BN, last);
       v.load(lds[buf ^ 1][1], k0 + BN, last);
     }
@@ -349,7 +411,7 @@ __global__ __launch_bounds__(256, (kWavesOf<T, DP>)) void attn_dq_k(BfAttnArgs a
     loads_done();
   }
   const float f = kScaled<T> ? (factor == 0.f ? 1.f : exp2f(-kPower<T>) / factor) : 1.f;
-  store_row<VEC>(out, dq, a.scale * f, half, a.dim, inside);
+  finish(a.scale * f);
 }
 
 // ---------------------------------------------------------------------------
@@ -414,8 +476,8 @@ __global__ __launch_bounds__((256 * DkvShape<T, DP>::kSplit), (DkvShape<T, DP>::
   const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6, part = wave >> 2;
   const Unit unit = unit_of(blockIdx.x, a.kv_heads);
   const int g = unit.head, group = a.heads / a.kv_heads;
-  const int slice = unit.number % a.slices;  // of the steps
-  Work w = find_tile(a, unit.number / a.slices, kK, a.causal);
+  const int slice = unit.number % a.query_slices;  // of the steps
+  Work w = find_tile(a, unit.number / a.query_slices, kK, a.causal);
   if (!w.any) return;
   if (a.causal) w.tile = (w.len - 1) / kK - w.tile;  // the first keys have most queries
   const int j0 = w.tile * kK, jl = (wave & 3) * 32 + (lane & 31), jw = j0 + (wave & 3) * 32, ji = j0 + jl;
@@ -425,7 +487,7 @@ __global__ __launch_bounds__((256 * DkvShape<T, DP>::kSplit), (DkvShape<T, DP>::
 #pragma unroll
   for (int i = 0; i < kDT; ++i) dk[i] = dv[i] = Acc{};
   const auto finish = [&]() __attribute__((always_inline)) {
-    if (a.slices == 1) {
+    if (a.query_slices == 1) {
       store_row<VEC>(static_cast<T*>(a.dk) + out, dk, 1.f, half, a.dim, inside);
       store_row<VEC>(static_cast<T*>(a.dv) + out, dv, 1.f, half, a.dim, inside);
     } else {
@@ -457,8 +519,8 @@ __global__ __launch_bounds__((256 * DkvShape<T, DP>::kSplit), (DkvShape<T, DP>::
   const int from = a.causal ? ji : 0;  // first query that sees the lane's key
   const int from_ds = a.causal ? max(ji, 1) : w.len == 1 ? 1 : 0;  // and has another: with one key dS is 0
   const int steps = (w.len - first + BM - 1) / BM, total = steps * group;
-  const int begin = static_cast<int>(static_cast<long>(total) * slice / a.slices);
-  const int end = static_cast<int>(static_cast<long>(total) * (slice + 1) / a.slices);
+  const int begin = static_cast<int>(static_cast<long>(total) * slice / a.query_slices);
+  const int end = static_cast<int>(static_cast<long>(total) * (slice + 1) / a.query_slices);
   typedef Loader<T, BM, DP, THREADS, VEC> Load;
   Load q(nullptr, a.q_row, a.dim), go(nullptr, a.do_row, a.dim);
   const auto fetch = [&](int h, int i0, int buf) __attribute__((always_inline)) {
@@ -569,29 +631,45 @@ __global__ __launch_bounds__((256 * DkvShape<T, DP>::kSplit), (DkvShape<T, DP>::
   finish();
 }
 
-// the slices' dk and dv, one behind the other, in a fixed order
+// the slices' gradients into one, in a fixed order: dq, or dk and dv, which lie
+// side by side in a slice
 template <typename T>
-__global__ __launch_bounds__(256) void attn_fold_k(T* dk, T* dv, const float* partial, long all, int slices) {
+__global__ __launch_bounds__(256) void attn_fold_k(T* first, T* second, const float* partial, long all, int slices) {
   const long i = (static_cast<long>(blockIdx.x) * 256 + threadIdx.x) * 4;
   if (i >= all) return;
   const int n = all - i < 4 ? static_cast<int>(all - i) : 4;
+  const long next = all * gridDim.y;
   partial += blockIdx.y * all + i;
   float sum[4] = {};
   for (int s = 0; s < slices; ++s)
 #pragma unroll
-    for (int u = 0; u < 4; ++u) sum[u] += u < n ? partial[2 * s * all + u] : 0.f;
-  T* out = (blockIdx.y ? dv : dk) + i;
+    for (int u = 0; u < 4; ++u) sum[u] += u < n ? partial[s * next + u] : 0.f;
+  T* out = (blockIdx.y ? second : first) + i;
 #pragma unroll
   for (int u = 0; u < 4; ++u)
     if (u < n) out[u] = static_cast<T>(sum[u]);
 }
 
+template <typename T>
+hipError_t fold(void* first, void* second, const float* partial, long all, int slices, hipStream_t stream) {
+  const long blocks = (all + 1023) / 1024;
+  if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(attn_fold_k<T>, dim3(blocks, second ? 2 : 1), dim3(256), 0, stream, static_cast<T*>(first),
+                     static_cast<T*>(second), partial, all, slices);
+  return hipGetLastError();
+}
+
 template <typename T, int DP, bool VEC>
 hipError_t fwd(const BfAttnArgs& a, hipStream_t stream) {
-  const long groups = units(most_tiles(a, 128), a.heads);
+  const long groups = units(most_tiles(a, 128) * a.key_slices, a.heads);
   if (groups > 0x7FFFFFFF) return hipErrorInvalidValue;
   if (a.drop.threshold) hipLaunchKernelGGL((attn_fwd_k<T, DP, VEC, true>), dim3(groups), dim3(256), 0, stream, a);
   else hipLaunchKernelGGL((attn_fwd_k<T, DP, VEC, false>), dim3(groups), dim3(256), 0, stream, a);
+  if (hipError_t e = hipGetLastError()) return e;
+  if (a.key_slices == 1) return hipSuccess;
+  const long blocks = (static_cast<long>(a.rows) * a.heads * ((a.dim + 3) / 4) + 255) / 256;
+  if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(attn_join_k<T>, dim3(blocks), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 
@@ -603,19 +681,19 @@ hipError_t fwd(const BfAttnArgs& a, hipStream_t stream) {
 
 template <typename T, int DP, bool VEC, bool DROP>
 hipError_t bwd(const BfAttnArgs& a, bool need_dkv, hipStream_t stream) {
-  const long groups = units(most_tiles(a, 128), a.heads), shared = units(most_tiles(a, 128) * a.slices, a.kv_heads);
+  const long groups = units(most_tiles(a, 128) * a.key_slices, a.heads);
+  const long shared = units(most_tiles(a, 128) * a.query_slices, a.kv_heads);
   if (groups > 0x7FFFFFFF || shared > 0x7FFFFFFF) return hipErrorInvalidValue;
   hipLaunchKernelGGL((attn_dq_k<T, DP, VEC, DROP>), dim3(groups), dim3(256), 0, stream, a);
   if (hipError_t e = hipGetLastError()) return e;
+  if (a.key_slices > 1)
+    if (hipError_t e = fold<T>(a.dq, nullptr, a.partial, static_cast<long>(a.rows) * a.heads * a.dim, a.key_slices, stream))
+      return e;
   if (!need_dkv) return hipSuccess;
   hipLaunchKernelGGL((attn_dkv_k<T, DP, VEC, DROP>), dim3(shared), dim3(256 * DkvShape<T, DP>::kSplit), 0, stream, a);
   if (hipError_t e = hipGetLastError()) return e;
-  if (a.slices == 1) return hipSuccess;
-  const long all = static_cast<long>(a.rows) * a.kv_heads * a.dim, blocks = (all + 1023) / 1024;
-  if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(attn_fold_k<T>, dim3(blocks, 2), dim3(256), 0, stream, static_cast<T*>(a.dk), static_cast<T*>(a.dv),
-                     a.partial, all, a.slices);
-  return hipGetLastError();
+  if (a.query_slices == 1) return hipSuccess;
+  return fold<T>(a.dk, a.dv, a.partial, static_cast<long>(a.rows) * a.kv_heads * a.dim, a.query_slices, stream);
 }
 
 template <typename T, int DP, bool VEC>
@@ -629,20 +707,37 @@ hipError_t bwd(const BfAttnArgs& a, bool need_dkv, hipStream_t stream) {
   return a.dim <= 64 ? bwd<T, 64, true>(a, need_dkv, stream) : bwd<T, 128, true>(a, need_dkv, stream);
 }
 
+int slices(long wanted, long most) {
+  const long n = wanted < most ? wanted : most;
+  return static_cast<int>(n < 1 ? 1 : n > 16 ? 16 : n);
+}
+
 }  // namespace
 
 extern "C" {
 
-// Slices of the queries in the dk and dv pass. A workgroup goes over all queries
-// of a head group, so few key heads or long sequences leave few workgroups; each
-// slice more costs 16 bytes of memory traffic for a value of dk and dv.
-int bf_attn_slices(const BfAttnArgs* a) {
+// Slices of the long axis: a workgroup goes over all keys of its rows, or (dk
+// and dv) over all queries of its keys and head group. Few tokens or few key
+// heads leave few workgroups, which then take a share of that axis each; a
+// second kernel joins the shares, from 32-bit sums in memory.
+int bf_attn_key_slices(const BfAttnArgs* a, int dtype) {
+  const long groups = (a->rows + 127L) / 128 * a->heads;
+  const long length = a->rows / (a->seqs > 0 ? a->seqs : 1);
+  return slices((BF_WANTQ + groups - 1) / groups, (length + 63) / 64 * (dtype == 0 ? 2 : 1) / 2);
+}
+
+int bf_attn_query_slices(const BfAttnArgs* a, int dtype) {
   const long groups = (a->rows + 127L) / 128 * a->kv_heads;
   const long length = a->rows / (a->seqs > 0 ? a->seqs : 1);
-  const long steps = (length + 63) / 64 * (a->heads / a->kv_heads);
-  const long wanted = (BF_WANT + groups - 1) / groups, most = steps / 4;
-  const long n = wanted < most ? wanted : most;
-  return static_cast<int>(n < 1 ? 1 : n > 16 ? 16 : n);
+  const long steps = (length + 63) / 64 * (a->heads / a->kv_heads) * (dtype == 0 ? 2 : 1);
+  return slices((BF_WANT + groups - 1) / groups, steps / 4);
+}
+
+long bf_attn_partial_floats(const BfAttnArgs* a) {
+  const long wide = static_cast<long>(a->rows) * a->heads, narrow = static_cast<long>(a->rows) * a->kv_heads;
+  const long keys = a->key_slices > 1 ? a->key_slices * wide * (a->dim + 1) : 0;
+  const long queries = a->query_slices > 1 ? a->query_slices * narrow * a->dim * 2 : 0;
+  return keys > queries ? keys : queries;
 }
 
 hipError_t bf_attn_fwd(const BfAttnArgs* a, int dtype, hipStream_t stream) {

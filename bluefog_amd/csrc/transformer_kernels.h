@@ -15,8 +15,8 @@ struct BfAttnArgs {
   void *o, *dq, *dk, *dv;  // written; contiguous [rows, heads, dim]
   float* lse;    // [heads, rows]; forward: written unless null
   float* delta;  // [heads, rows]; backward: written by dq, read by dk/dv
-  float* partial;  // [slices][dk, dv][rows, kv_heads, dim] where slices > 1
-  int slices;      // bf_attn_slices()
+  float* partial;  // bf_attn_partial_floats() of them
+  int key_slices, query_slices;  // of the axes that workgroups go along
   const int* cu;  // seqs + 1 ends of the sequences
   int seqs, rows, heads, kv_heads, dim;
   // element strides of a row and a head; the last dimension is dense
@@ -43,7 +43,9 @@ struct BfNormArgs {
 
 extern "C" {
 hipError_t bf_attn_fwd(const BfAttnArgs* a, int dtype, hipStream_t stream);
-int bf_attn_slices(const BfAttnArgs* a);
+int bf_attn_key_slices(const BfAttnArgs* a, int dtype);
+int bf_attn_query_slices(const BfAttnArgs* a, int dtype);
+long bf_attn_partial_floats(const BfAttnArgs* a);
 hipError_t bf_attn_bwd(const BfAttnArgs* a, int dtype, int need_dq,
                        int need_dkv, hipStream_t stream);
 hipError_t bf_norm_fwd(const BfNormArgs* a, int x_dtype, int r_dtype,

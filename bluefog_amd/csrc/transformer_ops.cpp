@@ -116,6 +116,14 @@ BfAttnArgs attn_args(const Tensor& q, const Tensor& k, const Tensor& v, const Te
   return a;
 }
 
+Tensor attn_partial(BfAttnArgs& a, const at::TensorOptions& f32) {
+  const long n = bf_attn_partial_floats(&a);
+  if (n == 0) return Tensor();
+  Tensor t = at::empty({n}, f32);
+  a.partial = t.data_ptr<float>();
+  return t;
+}
+
 Tensor attn_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu,
                     double scale, bool causal, const BfDropout& drop, Tensor* lse) {
   c10::DeviceGuard guard(q.device());
@@ -125,6 +133,9 @@ Tensor attn_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Ten
   BfAttnArgs a = attn_args(q, k, v, cu, scale, causal, drop);
   a.o = out.data_ptr();
   a.lse = lse ? lse->data_ptr<float>() : nullptr;
+  a.key_slices = bf_attn_key_slices(&a, code_of(q));
+  a.query_slices = 1;
+  const Tensor partial = attn_partial(a, q.options().dtype(at::kFloat));
   check(bf_attn_fwd(&a, code_of(q), stream_of(q)), "packed_attention");
   return out;
 }
@@ -173,12 +184,9 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
       a.dq = dq.data_ptr();
       a.dk = dk.data_ptr();
       a.dv = dv.data_ptr();
-      a.slices = bf_attn_slices(&a);
-      Tensor partial;
-      if (a.slices > 1 && need_dkv) {
-        partial = at::empty({a.slices, 2, dk.numel()}, lse.options());
-        a.partial = partial.data_ptr<float>();
-      }
+      a.key_slices = bf_attn_key_slices(&a, code_of(q));
+      a.query_slices = need_dkv ? bf_attn_query_slices(&a, code_of(q)) : 1;
+      const Tensor partial = attn_partial(a, lse.options());
       check(bf_attn_bwd(&a, code_of(q), need_dq, need_dkv, stream_of(q)), "packed_attention backward");
     }
     none[0] = dq, none[1] = dk, none[2] = dv;
