@@ -69,7 +69,7 @@ __global__ __launch_bounds__(256, (kWavesOf<T, DP>)) void attn_fwd_k(BfAttnArgs 
   const auto finish = [&](float f, float lse) __attribute__((always_inline)) {
     const long at = (row * a.heads + h) * a.dim, all = static_cast<long>(a.rows) * a.heads;
     if (a.key_slices == 1) {
-      store_row<VEC>(static_cast<T*>(a.o) + at, o, f, half, a.dim, inside);
+      store_row<VEC>(static_cast<T*>(a.o) + at, o, f, half, a.dim, inside, a.rest ? static_cast<T*>(a.rest) + at : nullptr);
       if (a.lse && inside && half == 0) a.lse[static_cast<long>(h) * a.rows + row] = lse;
     } else {
       store_row<VEC>(a.partial + slice * all * a.dim + at, o, f, half, a.dim, inside);
@@ -250,15 +250,23 @@ __global__ __launch_bounds__(256) void attn_join_k(BfAttnArgs a) {
     for (int u = 0; u < 4; ++u) out[u] += share * x[u];
   }
   T* o = static_cast<T*>(a.o) + at * a.dim + c;
+  T* rest = a.rest ? static_cast<T*>(a.rest) + at * a.dim + c : nullptr;
 #pragma unroll
   for (int u = 0; u < 4; ++u)
-    if (u < n) o[u] = static_cast<T>(out[u] / total);
+    if (u < n) {
+      out[u] /= total;
+      o[u] = static_cast<T>(out[u]);
+      if (rest) rest[u] = static_cast<T>(out[u] - static_cast<float>(o[u]));
+    }
   if (a.lse && c == 0) a.lse[at % a.heads * a.rows + at / a.heads] = top + log2f(total);
 }
 
 // ---------------------------------------------------------------------------
 // backward, dq: the same loop as forward, with dP^T = v dO^T beside S^T, and
-// dq^T = k^T dS^T. Its first act is delta, which the other kernel reads.
+// dq^T = k^T dS^T. Its first act is delta, which the other kernel reads: from O
+// as it was before it was rounded (the forward pass keeps the rest, in the same
+// type), since delta's error goes into all dS of a row at once. With the rounded
+// O, dq and dk were 1.6 times as far off as the rounding of P and dS makes them.
 //
 // f16 would lose small dS and overflow with large ones, whatever dO's size.
 // Its dS is held times a power of two of its own for each lane's row (or key),
@@ -340,6 +348,7 @@ __global__ __launch_bounds__(256, (kWavesOf<T, DP>)) void attn_dq_k(BfAttnArgs a
     const T* q = static_cast<const T*>(a.q) + row * a.q_row + h * a.q_head;
     const T* go = static_cast<const T*>(a.dout) + row * a.do_row + h * a.do_head;
     const T* o = static_cast<const T*>(a.out) + (row * a.heads + h) * a.dim;
+    const T* rest = a.rest ? static_cast<const T*>(a.rest) + (row * a.heads + h) * a.dim : nullptr;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       qf[s] = load_row<VEC>(q, s, half, a.dim);
@@ -347,6 +356,11 @@ __global__ __launch_bounds__(256, (kWavesOf<T, DP>)) void attn_dq_k(BfAttnArgs a
       const Frag<T> of = load_row<VEC>(o, s, half, a.dim);
 #pragma unroll
       for (int i = 0; i < 8; ++i) delta += static_cast<float>(gf[s][i]) * static_cast<float>(of[i]);
+      if (rest) {
+        const Frag<T> rf = load_row<VEC>(rest, s, half, a.dim);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) delta += static_cast<float>(gf[s][i]) * static_cast<float>(rf[i]);
+      }
     }
     delta += swap_halves(delta);
   }

@@ -218,9 +218,10 @@ __device__ __forceinline__ Frag<T> load_row(const T* row, int step, int half, in
 
 // accumulators [columns of the row on 32 * tiles][one row a lane] times f into
 // memory: 16 bytes a lane. The halves hold quads of columns; a swap gives each
-// eight in a row.
+// eight in a row. What the rounding took goes to `rest` unless that is null.
 template <bool VEC, typename T, int TILES>
-__device__ __forceinline__ void store_row(T* row, Acc (&acc)[TILES], float f, int half, int dim, bool inside) {
+__device__ __forceinline__ void store_row(T* row, Acc (&acc)[TILES], float f, int half, int dim, bool inside,
+                                          T* rest = nullptr) {
 #pragma unroll
   for (int dt = 0; dt < TILES; ++dt)
 #pragma unroll
@@ -237,15 +238,22 @@ __device__ __forceinline__ void store_row(T* row, Acc (&acc)[TILES], float f, in
       }
       const int c = dt * 32 + s * 16 + half * 8;
       if (!inside) continue;
-      T t[8];
+      T t[8], less[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) t[i] = static_cast<T>(x[i]);
+      for (int i = 0; i < 8; ++i) {
+        t[i] = static_cast<T>(x[i]);
+        less[i] = static_cast<T>(x[i] - static_cast<float>(t[i]));
+      }
       if (VEC && c + 8 <= dim) {
         __builtin_memcpy(row + c, t, sizeof(t));
+        if (rest) __builtin_memcpy(rest + c, less, sizeof(less));
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (c + i < dim) row[c + i] = t[i];
+          if (c + i < dim) {
+            row[c + i] = t[i];
+            if (rest) rest[c + i] = less[i];
+          }
       }
     }
 }

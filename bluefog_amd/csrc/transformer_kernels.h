@@ -13,6 +13,7 @@ struct BfAttnArgs {
   const void *q, *k, *v, *dout;
   const void* out;  // backward: the forward's output
   void *o, *dq, *dk, *dv;  // written; contiguous [rows, heads, dim]
+  void* rest;    // what rounding took from o, [rows, heads, dim]; may be null
   float* lse;    // [heads, rows]; forward: written unless null
   float* delta;  // [heads, rows]; backward: written by dq, read by dk/dv
   float* partial;  // bf_attn_partial_floats() of them

@@ -125,14 +125,16 @@ Tensor attn_partial(BfAttnArgs& a, const at::TensorOptions& f32) {
 }
 
 Tensor attn_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu,
-                    double scale, bool causal, const BfDropout& drop, Tensor* lse) {
+                    double scale, bool causal, const BfDropout& drop, Tensor* lse, Tensor* rest) {
   c10::DeviceGuard guard(q.device());
   Tensor out = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
   if (lse) *lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
+  if (rest && q.scalar_type() != at::kFloat) *rest = at::empty(out.sizes(), q.options());
   if (out.numel() == 0) return out;
   BfAttnArgs a = attn_args(q, k, v, cu, scale, causal, drop);
   a.o = out.data_ptr();
   a.lse = lse ? lse->data_ptr<float>() : nullptr;
+  a.rest = rest && rest->defined() ? rest->data_ptr() : nullptr;
   a.key_slices = bf_attn_key_slices(&a, code_of(q));
   a.query_slices = 1;
   const Tensor partial = attn_partial(a, q.options().dtype(at::kFloat));
@@ -144,10 +146,10 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
                         const Tensor& cu, const std::optional<Tensor>& seed_tensor, double scale,
                         bool causal, double p, int64_t seed, int64_t offset) {
-    Tensor lse;
+    Tensor lse, rest;
     const Tensor st = seed_tensor.value_or(Tensor());
-    Tensor out = attn_forward(q, k, v, cu, scale, causal, dropout_args(st, seed, offset, p), &lse);
-    ctx->save_for_backward({q, k, v, cu, st, out, lse});
+    Tensor out = attn_forward(q, k, v, cu, scale, causal, dropout_args(st, seed, offset, p), &lse, &rest);
+    ctx->save_for_backward({q, k, v, cu, st, out, lse, rest});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["p"] = p;
@@ -161,7 +163,7 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
     variable_list none(10);
     if (!grads[0].defined()) return none;
     const variable_list s = ctx->get_saved_variables();
-    const Tensor &q = s[0], &k = s[1], &v = s[2], &cu = s[3], &seed_tensor = s[4], &out = s[5], &lse = s[6];
+    const Tensor &q = s[0], &k = s[1], &v = s[2], &cu = s[3], &seed_tensor = s[4], &out = s[5], &lse = s[6], &rest = s[7];
     c10::DeviceGuard guard(q.device());
     const bool need_dq = ctx->needs_input_grad(0);
     const bool need_dkv = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
@@ -177,6 +179,7 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
                                             ctx->saved_data["offset"].toInt(),
                                             ctx->saved_data["p"].toDouble()));
       a.out = out.const_data_ptr();
+      a.rest = rest.defined() ? const_cast<void*>(rest.const_data_ptr()) : nullptr;
       a.dout = dout.const_data_ptr();
       a.do_row = dout.stride(0), a.do_head = dout.stride(1);
       a.lse = lse.data_ptr<float>();
@@ -218,7 +221,7 @@ Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
   py::gil_scoped_release nogil;
   const Tensor rq = readable(q), rk = readable(k), rv = readable(v);
   if (grad) return PackedAttention::apply(rq, rk, rv, cu, seed_tensor, scale, causal, p, seed, offset);
-  return attn_forward(rq, rk, rv, cu, scale, causal, dropout_args(st, seed, offset, p), nullptr);
+  return attn_forward(rq, rk, rv, cu, scale, causal, dropout_args(st, seed, offset, p), nullptr, nullptr);
 }
 
 // ---------------------------------------------------------------------------
