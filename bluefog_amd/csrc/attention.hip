@@ -31,7 +31,10 @@ constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;  // keys of a tile
 
 // waves of a SIMD whose registers the kernels are held to
 template <typename T, int DP>
-constexpr int kWavesOf = sizeof(T) == 2 && DP == 64 ? 3 : 2;
+constexpr int kFwdWaves = sizeof(T) == 2 && DP == 64 ? 3 : 2;
+// f32 under two waves of heads of 128 spills: 3.9 ms where it takes 1.8 (8192 tokens, 16 heads)
+template <typename T, int DP>
+constexpr int kDqWaves = sizeof(T) == 4 && DP == 128 ? 1 : kFwdWaves<T, DP>;
 
 // a slice's keys of `keys`, whole tiles
 __device__ __forceinline__ int2 keys_of(int keys, int tile, int slice, int slices) {
@@ -49,7 +52,7 @@ struct Mode {
 constexpr float kSlack = 8.f;
 
 template <typename T, int DP, bool VEC, bool DROP>
-__global__ __launch_bounds__(256, (kWavesOf<T, DP>)) void attn_fwd_k(BfAttnArgs a) {
+__global__ __launch_bounds__(256, (kFwdWaves<T, DP>)) void attn_fwd_k(BfAttnArgs a) {
   constexpr int kQ = 128, BN = kKeys<T>, kSub = BN / 32, kSteps = DP / 16, kDT = DP / 32;
   typedef Tile<T, BN, DP, 256, VEC> KV;
   __shared__ __align__(1024) char lds[2][2][KV::kBytes];
@@ -301,7 +304,7 @@ __device__ __forceinline__ void rescale(Acc (&acc)[TILES], float& factor, const 
 }
 
 template <typename T, int DP, bool VEC, bool DROP>
-__global__ __launch_bounds__(256, (kWavesOf<T, DP>)) void attn_dq_k(BfAttnArgs a) {
+__global__ __launch_bounds__(256, (kDqWaves<T, DP>)) void attn_dq_k(BfAttnArgs a) {
   constexpr int kQ = 128, BN = kKeys<T>, kSub = BN / 32, kSteps = DP / 16, kDT = DP / 32;
   typedef Tile<T, BN, DP, 256, VEC> KV;
   __shared__ __align__(1024) char lds[2][2][KV::kBytes];

@@ -180,12 +180,18 @@ struct Loader {
         }
       }
     } else {
+      // rows that do not start on 16 bytes: through registers, unaligned
       const uint32_t most = (last - first) * step;
-      for (uint32_t i = threadIdx.x; i < ROWS * DP; i += THREADS) {
-        const int r = i / DP, c = i % DP;
-        if (c < dim)
-          *reinterpret_cast<T*>(lds + Of::at(r, c / Of::kEach) + (c % Of::kEach) * sizeof(T)) =
-              *reinterpret_cast<const T*>(from + min(r * step, most) + c * sizeof(T));
+#pragma unroll 4
+      for (uint32_t off = threadIdx.x * 16; off < Of::kBytes; off += THREADS * 16) {
+        const int r = off / Of::kRowBytes, c = (off % Of::kRowBytes >> 4) * Of::kEach;
+        const T* values = reinterpret_cast<const T*>(from + min(r * step, most)) + c;
+        T got[Of::kEach];
+        if (c + Of::kEach <= dim) __builtin_memcpy(got, values, 16);
+        else
+#pragma unroll
+          for (int u = 0; u < Of::kEach; ++u) got[u] = c + u < dim ? values[u] : static_cast<T>(0.f);
+        __builtin_memcpy(__builtin_assume_aligned(lds + Of::at(r, c / Of::kEach), 16), got, 16);
       }
     }
   }
@@ -202,16 +208,12 @@ template <bool VEC, typename T>
 __device__ __forceinline__ Frag<T> load_row(const T* row, int step, int half, int dim) {
   Frag<T> f;
   const int c = step * 16 + half * 8;
-  if (VEC && c < dim) {
-    if (sizeof(T) == 4 && dim - c < 8) {  // f32: four of eight
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = i < 4 ? row[c + i] : static_cast<T>(0.f);
-    } else {
-      __builtin_memcpy(&f, row + c, sizeof(f));
-    }
+  if (c + 8 <= dim) {
+    __builtin_memcpy(&f, row + c, sizeof(f));
   } else {
+    // whole 16 bytes of halves; of f32, four of eight
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = !VEC && c + i < dim ? row[c + i] : static_cast<T>(0.f);
+    for (int i = 0; i < 8; ++i) f[i] = (!VEC || (sizeof(T) == 4 && i < 4)) && c + i < dim ? row[c + i] : static_cast<T>(0.f);
   }
   return f;
 }
@@ -244,7 +246,7 @@ __device__ __forceinline__ void store_row(T* row, Acc (&acc)[TILES], float f, in
         t[i] = static_cast<T>(x[i]);
         less[i] = static_cast<T>(x[i] - static_cast<float>(t[i]));
       }
-      if (VEC && c + 8 <= dim) {
+      if (c + 8 <= dim) {
         __builtin_memcpy(row + c, t, sizeof(t));
         if (rest) __builtin_memcpy(rest + c, less, sizeof(less));
       } else {
@@ -302,9 +304,8 @@ struct Work {
 };
 
 __device__ __forceinline__ int2 bounds_of(const BfAttnArgs& a, int seq) {
-  int begin = min(max(a.cu[seq], 0), a.rows);
-  int end = seq < a.seqs ? min(max(a.cu[seq + 1], begin), a.rows) : a.rows;
-  return make_int2(begin, end);
+  const int begin = min(max(a.cu[seq], 0), a.rows), next = a.cu[min(seq + 1, a.seqs)];
+  return make_int2(begin, seq < a.seqs ? min(max(next, begin), a.rows) : a.rows);
 }
 
 __device__ __forceinline__ int wave_sum(int x) {
@@ -349,11 +350,12 @@ __device__ __forceinline__ Work find_tile(const BfAttnArgs& a, int number, int s
     int first = 0, count = n, chunk = (n + 63) / 64;
     while (true) {
       int mine = 0;
-      for (int i = 0; i < chunk; ++i)
-        if (lane * chunk + i < count) {
-          const int2 b = bounds_of(a, first + lane * chunk + i);
-          mine += (b.y - b.x + size - 1) / size;
-        }
+#pragma unroll 8
+      for (int i = 0; i < chunk; ++i) {  // unguarded, so that the loads go out together
+        const int at = lane * chunk + i;
+        const int2 b = bounds_of(a, first + min(at, count - 1));
+        mine += at < count ? (b.y - b.x + size - 1) / size : 0;
+      }
       const int upto = sum_up_to(mine);
       const unsigned long long past = __ballot(upto > number);
       if (!past) return w;
