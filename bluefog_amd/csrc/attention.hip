@@ -52,7 +52,7 @@ struct Mode {
 constexpr float kSlack = 8.f;
 
 template <typename T, int DP, bool VEC, bool DROP>
-__global__ __launch_bounds__(256, (kFwdWaves<T, DP>)) void attn_fwd_k(BfAttnArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kFwdWaves<T, DP>, kFwdWaves<T, DP>))) void attn_fwd_k(BfAttnArgs a) {
   constexpr int kQ = 128, BN = kKeys<T>, kSub = BN / 32, kSteps = DP / 16, kDT = DP / 32;
   typedef Tile<T, BN, DP, 256, VEC> KV;
   __shared__ __align__(1024) char lds[2][2][KV::kBytes];
@@ -304,7 +304,7 @@ __device__ __forceinline__ void rescale(Acc (&acc)[TILES], float& factor, const 
 }
 
 template <typename T, int DP, bool VEC, bool DROP>
-__global__ __launch_bounds__(256, (kDqWaves<T, DP>)) void attn_dq_k(BfAttnArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kDqWaves<T, DP>, kDqWaves<T, DP>))) void attn_dq_k(BfAttnArgs a) {
   constexpr int kQ = 128, BN = kKeys<T>, kSub = BN / 32, kSteps = DP / 16, kDT = DP / 32;
   typedef Tile<T, BN, DP, 256, VEC> KV;
   __shared__ __align__(1024) char lds[2][2][KV::kBytes];
@@ -445,23 +445,19 @@ __global__ __launch_bounds__(256, (kDqWaves<T, DP>)) void attn_dq_k(BfAttnArgs a
 //         sums meet in LDS at the end
 //   V_IN_LDS: v's fragments are read again rather than kept in registers
 //   WAVES of a SIMD whose registers it is held to
-template <typename T, int DP>
+//
+// Heads of 128: the sums take 128 registers. Eight waves, two to a SIMD, reach
+// 670 TFLOP/s (16384 tokens, 16 heads, bf16) and four with all registers 630;
+// the masks of dropout do not fit beside the sums of two, so there it is
+// four: 450 against 330 TFLOP/s (sequences of 512).
+template <typename T, int DP, bool DROP>
 struct DkvShape {
-  static constexpr int kSplit = 1, kSubs = sizeof(T) == 2 ? 2 : 1, kWaves = 2;
-  static constexpr bool kVInLds = false;
+  static constexpr bool kHalf = sizeof(T) == 2, kWide = DP == 128;
+  static constexpr int kSplit = kHalf && kWide && !DROP ? 2 : 1;
+  static constexpr int kSubs = kHalf && kSplit == 1 ? 2 : 1;  // f32: LDS holds 32 queries a step
+  static constexpr int kWaves = kWide && kSplit == 1 ? 1 : 2;
+  static constexpr bool kVInLds = kWide && !(kHalf && DROP);
 };
-template <typename T>
-struct DkvShape<T, 128> {
-  static constexpr int kSplit = 2, kSubs = 1, kWaves = 2;
-  static constexpr bool kVInLds = true;
-};
-template <>
-struct DkvShape<float, 128> {  // LDS holds 32 queries a step
-  static constexpr int kSplit = 1, kSubs = 1, kWaves = 1;
-  static constexpr bool kVInLds = true;
-};
-template <typename T, int DP>
-constexpr int kDkvQueries = 32 * DkvShape<T, DP>::kSplit * DkvShape<T, DP>::kSubs;  // of a step
 
 // the sums of the second four waves to those of the first, through LDS
 template <int TILES>
@@ -479,9 +475,11 @@ __device__ __forceinline__ void join(Acc (&acc)[TILES], void* lds, int part) {
 }
 
 template <typename T, int DP, bool VEC, bool DROP>
-__global__ __launch_bounds__((256 * DkvShape<T, DP>::kSplit), (DkvShape<T, DP>::kWaves)) void attn_dkv_k(BfAttnArgs a) {
-  typedef DkvShape<T, DP> Shape;
-  constexpr int kK = 128, SPLIT = Shape::kSplit, SUBS = Shape::kSubs, THREADS = 256 * SPLIT, BM = kDkvQueries<T, DP>;
+__global__ __launch_bounds__((256 * DkvShape<T, DP, DROP>::kSplit))
+__attribute__((amdgpu_waves_per_eu(DkvShape<T, DP, DROP>::kWaves, DkvShape<T, DP, DROP>::kWaves))) void attn_dkv_k(BfAttnArgs a) {
+  typedef DkvShape<T, DP, DROP> Shape;
+  constexpr int kK = 128, SPLIT = Shape::kSplit, SUBS = Shape::kSubs, THREADS = 256 * SPLIT;
+  constexpr int BM = 32 * SPLIT * SUBS;  // queries of a step
   constexpr int kSteps = DP / 16, kDT = DP / 32;
   constexpr bool V_IN_LDS = Shape::kVInLds;
   typedef Tile<T, BM, DP, THREADS, VEC> QG;
@@ -572,6 +570,7 @@ __global__ __launch_bounds__((256 * DkvShape<T, DP>::kSplit), (DkvShape<T, DP>::
         for (int i = 0; i < kSteps; ++i)
           dp = mma(QG::read_row(lds[buf][1], sub + (lane & 31), i, half),
                    V_IN_LDS ? Values::read_row(v_lds, jl, i, half) : vf[V_IN_LDS ? 0 : i], dp);
+        if (sizeof(T) == 2) feed<V_IN_LDS ? 8 : 6, 2 * kSteps, V_IN_LDS ? 2 : 1>();
         if (DROP) {
           // the lane's share of a query's mask, as the forward pass has it
           uint32_t bits = 0;
@@ -630,6 +629,7 @@ __global__ __launch_bounds__((256 * DkvShape<T, DP>::kSplit), (DkvShape<T, DP>::
             dk[i] = mma(QG::read_columns(lds[buf][0], sub + t * 16, i, lane), df, dk[i]);
           }
         }
+        if (sizeof(T) == 2) feed<8, 4 * kDT, 2>();
       }
     }
     loads_done();
@@ -712,7 +712,7 @@ hipError_t bwd(const BfAttnArgs& a, bool need_dkv, hipStream_t stream) {
     if (hipError_t e = fold<T>(a.dq, nullptr, a.partial, static_cast<long>(a.rows) * a.heads * a.dim, a.key_slices, stream))
       return e;
   if (!need_dkv) return hipSuccess;
-  hipLaunchKernelGGL((attn_dkv_k<T, DP, VEC, DROP>), dim3(shared), dim3(256 * DkvShape<T, DP>::kSplit), 0, stream, a);
+  hipLaunchKernelGGL((attn_dkv_k<T, DP, VEC, DROP>), dim3(shared), dim3(256 * DkvShape<T, DP, DROP>::kSplit), 0, stream, a);
   if (hipError_t e = hipGetLastError()) return e;
   if (a.query_slices == 1) return hipSuccess;
   return fold<T>(a.dk, a.dv, a.partial, static_cast<long>(a.rows) * a.kv_heads * a.dim, a.query_slices, stream);

@@ -203,6 +203,30 @@ __device__ __forceinline__ void loads_done() {
   __syncthreads();
 }
 
+// The order of a stretch of matrix products and the LDS reads that feed them:
+// AHEAD reads first, then a product and EACH reads in turn. Left to itself the
+// compiler reads one fragment at a time and waits for it, four times as long as
+// the product takes.
+template <int AHEAD, int PRODUCTS, int EACH>
+__device__ __forceinline__ void feed() {
+  __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+  for (int i = 0; i < PRODUCTS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, EACH, 0);
+  }
+}
+
+template <int PRODUCTS, int READS, int VALU>
+__device__ __forceinline__ void weave() {
+#pragma unroll
+  for (int i = 0; i < PRODUCTS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    if (VALU) __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
+  }
+}
+
 // fragment of a row in memory, columns of step `step`; 0 behind dim
 template <bool VEC, typename T>
 __device__ __forceinline__ Frag<T> load_row(const T* row, int step, int half, int dim) {
