@@ -2,7 +2,11 @@
 """BERT-base encoder with a masked-LM head — for BASELINE config 5
 (seqlen-512 hierarchical neighbor_allreduce). Standard architecture,
 self-contained; uses torch's fused scaled_dot_product_attention, which on
-ROCm lowers to the MIOpen/CK flash-attention path."""
+ROCm lowers to the MIOpen/CK flash-attention path.
+
+A batch can also be packed: its sequences one behind the other, without
+padding, and ``cu_seqlens`` with their ends. Attention, norms and dropout then
+run in bluefog_amd's own operators (ops/transformer.py)."""
 
 
 
@@ -58,6 +62,17 @@ class BertEmbeddings(nn.Module):
         )
         return self.dropout(self.norm(x))
 
+    def packed(self, input_ids, cu_seqlens, p, seed):
+        from bluefog_amd.ops.transformer import counter_dropout, layer_norm
+
+        token = torch.arange(input_ids.shape[0], device=input_ids.device, dtype=cu_seqlens.dtype)
+        sequence = torch.searchsorted(cu_seqlens, token, right=True) - 1
+        # rows behind the last sequence may lie further than the table goes
+        pos = (token - cu_seqlens[sequence]).clamp_max(self.position.num_embeddings - 1)
+        x = self.word(input_ids) + self.position(pos) + self.token_type(torch.zeros_like(input_ids))
+        x = layer_norm(x, self.norm.weight, self.norm.bias, self.norm.eps)
+        return counter_dropout(x, p, seed) if p else x
+
 
 class BertSelfAttention(nn.Module):
     def __init__(self, cfg: BertConfig):
@@ -76,6 +91,13 @@ class BertSelfAttention(nn.Module):
             q, k, v, dropout_p=self.dropout_p if self.training else 0.0
         )
         return self.out(o.transpose(1, 2).reshape(B, S, H))
+
+    def packed(self, x, cu_seqlens, p, seed, offset):
+        from bluefog_amd.ops.transformer import packed_attention
+
+        q, k, v = self.qkv(x).view(x.shape[0], 3, self.nh, self.hd).unbind(1)
+        o = packed_attention(q, k, v, cu_seqlens, dropout_p=p, seed=seed, offset=offset)
+        return self.out(o.view(x.shape[0], -1))
 
 
 class BertLayer(nn.Module):
@@ -98,6 +120,18 @@ class BertLayer(nn.Module):
         x = self.norm1(self.dropout(self.attn(x)), x)
         return self.norm2(self.dropout(self.mlp(x)), x)
 
+    def packed(self, x, cu_seqlens, p, seed, offset):
+        """One block on a packed batch; its masks have offsets ``offset`` to
+        ``offset + 2``."""
+        from bluefog_amd.ops.transformer import layer_norm
+
+        def join(norm, y, x, offset):
+            return layer_norm(y, norm.weight, norm.bias, norm.eps, residual=x,
+                              dropout_p=p, seed=seed, offset=offset)
+
+        x = join(self.norm1, self.attn.packed(x, cu_seqlens, p, seed, offset), x, offset + 1)
+        return join(self.norm2, self.mlp(x), x, offset + 2)
+
 
 class BertForMaskedLM(nn.Module):
     def __init__(self, cfg: BertConfig):
@@ -116,16 +150,49 @@ class BertForMaskedLM(nn.Module):
             if isinstance(m, nn.Linear) and m.bias is not None:
                 nn.init.zeros_(m.bias)
 
-    def forward(self, input_ids, labels=None):
-        x = self.embeddings(input_ids)
-        for layer in self.layers:
-            x = layer(x)
+    def forward(self, input_ids, labels=None, cu_seqlens=None):
+        """``input_ids`` [batch, length], or [tokens] with ``cu_seqlens``
+        (int32, 0 and the end of every sequence). A ``cu_seqlens`` on the CPU is
+        checked and moved; one on the GPU is taken as it is, so that no step
+        waits for it: its sequences have to fit the position table. Tokens
+        behind the last sequence cost their share and mean nothing: label them
+        -100."""
+        if cu_seqlens is None:
+            x = self.embeddings(input_ids)
+            for layer in self.layers:
+                x = layer(x)
+        else:
+            x = self._packed(input_ids, cu_seqlens)
         logits = self.head(x)
         if labels is not None:
             return F.cross_entropy(
                 logits.view(-1, self.cfg.vocab_size), labels.view(-1), ignore_index=-100
             )
         return logits
+
+    def _packed(self, input_ids, cu_seqlens):
+        if input_ids.dim() != 1:
+            raise ValueError("a packed batch is one row of tokens")
+        if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+            raise ValueError("cu_seqlens has to be an int32 vector")
+        if not cu_seqlens.is_cuda:
+            ends = cu_seqlens.tolist()
+            lengths = [b - a for a, b in zip(ends, ends[1:])]
+            if ends[0] != 0 or ends[-1] > input_ids.shape[0] or any(n < 0 for n in lengths):
+                raise ValueError("cu_seqlens has to rise from 0 to at most the number of tokens")
+            if max(lengths, default=0) > self.cfg.max_position_embeddings:
+                raise ValueError(
+                    f"a sequence of {max(lengths)} tokens does not fit "
+                    f"{self.cfg.max_position_embeddings} positions"
+                )
+            cu_seqlens = cu_seqlens.to(input_ids.device)
+        p = self.cfg.dropout if self.training else 0.0
+        # one seed for a step; every mask of it has an offset of its own
+        seed = torch.randint(1 << 62, (1,), device=input_ids.device) if p else None
+        x = self.embeddings.packed(input_ids, cu_seqlens, p, seed)
+        for i, layer in enumerate(self.layers):
+            x = layer.packed(x, cu_seqlens, p, seed, 1 + 3 * i)
+        return x
 
 
 def bert_base():

@@ -1,0 +1,149 @@
+# Copyright 2026. Licensed under the Apache License, Version 2.0.
+"""BERT on packed batches: packed attention, layer norm and counter-based
+dropout together, as a model runs them."""
+
+import copy
+
+import pytest
+import torch
+
+from bluefog_amd import models
+
+
+def _tiny_bert(dropout=0.0):
+    torch.manual_seed(3)
+    return models.BertForMaskedLM(
+        models.BertConfig(vocab_size=97, hidden_size=64, num_hidden_layers=2, num_attention_heads=4,
+                          intermediate_size=128, max_position_embeddings=40, dropout=dropout)
+    )
+
+
+def _packed_batch(device):
+    lengths = [7, 40, 1, 0, 23]
+    g = torch.Generator().manual_seed(5)
+    ids = torch.randint(0, 97, (sum(lengths) + 3,), generator=g)
+    labels = torch.where(torch.rand(ids.shape, generator=g) < 0.3, ids, -100)
+    labels[sum(lengths):] = -100
+    cu = torch.tensor([0] + lengths).cumsum(0).to(torch.int32)
+    return lengths, ids.to(device), labels.to(device), cu
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_bert_packed_matches_its_sequences_alone(device):
+    """Logits, loss and gradients of a packed batch against the dense model on
+    each sequence by itself, in 64 bits. The packed run is 32-bit: two blocks of
+    sums of at most 128 terms around values of size 1 keep six digits of the
+    largest."""
+    model = _tiny_bert().to(device)
+    lengths, ids, labels, cu = _packed_batch(device)
+    exact = copy.deepcopy(model).cpu().double()
+    logits, at = [], 0
+    for n in lengths:
+        if n:
+            logits.append(exact(ids[None, at:at + n].cpu())[0])
+        at += n
+    logits = torch.cat(logits)
+    loss = torch.nn.functional.cross_entropy(logits, labels[:at].cpu(), ignore_index=-100)
+    loss.backward()
+    got = model(ids, cu_seqlens=cu)
+    assert (got[:at].cpu().double() - logits).abs().max() < 1e-5 * logits.abs().max()
+    got = model(ids, labels=labels, cu_seqlens=cu)
+    assert abs(got.item() - loss.item()) < 1e-5 * loss.item()
+    got.backward()
+    for a, b in zip(model.parameters(), exact.parameters()):
+        assert (a.grad.cpu().double() - b.grad).abs().max() <= 2e-5 * b.grad.abs().max() + 1e-9
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_bert_packed_dropout(device):
+    """Masks follow torch's seed; evaluation has none; every gradient is there."""
+    model = _tiny_bert(0.2).to(device)
+    lengths, ids, labels, cu = _packed_batch(device)
+    used = slice(0, sum(lengths))
+
+    def run():
+        torch.manual_seed(11)
+        return model(ids, cu_seqlens=cu.to(device))[used]
+
+    first = run()
+    assert torch.equal(first, run())
+    assert not torch.equal(first, model(ids, cu_seqlens=cu)[used])
+    loss = model(ids, labels=labels, cu_seqlens=cu)
+    loss.backward()
+    assert all(torch.isfinite(p.grad).all() for p in model.parameters())
+    model.eval()
+    quiet = model(ids, cu_seqlens=cu)[used]
+    assert torch.equal(quiet, model(ids, cu_seqlens=cu)[used])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_bert_packed_half_precision(dtype):
+    """Under autocast the residual stream is 32-bit under half-precision
+    branches; a model of that type runs as well. Both stay within the type's
+    roundings of the 32-bit run: u = eps / 2 of values of size 4 at each of
+    eight roundings of the two blocks and the head, whose width of 64 makes the
+    errors of independent terms add up like their root, and a factor of 4."""
+    model = _tiny_bert().cuda().eval()
+    lengths, ids, _, cu = _packed_batch("cuda")
+    used = slice(0, sum(lengths))
+    with torch.no_grad():
+        want = model(ids, cu_seqlens=cu)[used]
+        with torch.autocast("cuda", dtype=dtype):
+            a = model(ids, cu_seqlens=cu)[used]
+        b = copy.deepcopy(model).to(dtype)(ids, cu_seqlens=cu)[used]
+    bound = torch.finfo(dtype).eps / 2 * 4 * 8 * 4
+    assert (a.float() - want).abs().max() < bound and (b.float() - want).abs().max() < bound
+
+
+@pytest.mark.gpu
+def test_bert_packed_in_a_captured_step():
+    """A captured training step against the eager one, with new tokens, labels
+    and lengths at every replay."""
+    model = _tiny_bert().cuda()
+    lengths, ids, labels, cu = _packed_batch("cuda")
+    cu = cu.cuda()
+    params = list(model.parameters())
+
+    def step():
+        loss = model(ids, labels=labels, cu_seqlens=cu)
+        return [loss.detach(), *torch.autograd.grad(loss, params)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for n in range(4):
+        ids.copy_(torch.randint(0, 97, ids.shape))
+        labels.copy_(torch.where(torch.rand(ids.shape) < 0.5, torch.randint(0, 97, ids.shape), -100))
+        cu.copy_(torch.tensor([0, 3 + n, 30, 30, 55, 60 + n]))
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = [t.clone() for t in got]
+        # the library's sums over the embeddings' rows have no fixed order
+        for a, b in zip(replayed, step()):
+            assert (a - b).abs().max() <= 1e-5 * b.abs().max() + 1e-8
+
+
+def test_bert_packed_refusals():
+    model = _tiny_bert()
+    ids = torch.zeros(50, dtype=torch.int64)
+
+    def refused(match, ids, cu):
+        with pytest.raises(ValueError, match=match):
+            model(ids, cu_seqlens=cu)
+
+    def ends(*v):
+        return torch.tensor(v, dtype=torch.int32)
+
+    refused("one row", ids[None], ends(0, 50))
+    refused("int32", ids, ends(0, 30).long())
+    refused("rise", ids, ends(0, 51))
+    refused("rise", ids, ends(0, 20, 10))
+    refused("rise", ids, ends(1, 20))
+    refused("does not fit", ids, ends(0, 41))
