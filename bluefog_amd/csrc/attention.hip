@@ -118,6 +118,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kFwdWaves<T
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) s[u] = mma(KV::read_row(lds[buf][0], u * 32 + (lane & 31), i, half), qf[i], s[u]);
     }
+    if (sizeof(T) == 2) feed<4, kSub * kSteps, 1>();
     if (MASKED) {
 #pragma unroll
       for (int u = 0; u < kSub; ++u)
@@ -145,13 +146,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kFwdWaves<T
     for (int u = 0; u < BN / 16; ++u) {
       uint4 bits;
       if (DROP) bits = bf_philox((k0 / 16 + u) * 2 + half, static_cast<uint32_t>(row), h, a.drop.offset, key);
+      float x[8];
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
-        float x = __builtin_amdgcn_exp2f(s[u / 2][(u & 1) * 8 + r] * c - base);
-        l += x;
-        if (DROP) x = bf_half(bits, r) >= a.drop.threshold ? x : 0.f;
-        p[u][r] = static_cast<T>(x);
+        x[r] = __builtin_amdgcn_exp2f(s[u / 2][(u & 1) * 8 + r] * c - base);
+        l += x[r];
+        if (DROP) x[r] = bf_half(bits, r) >= a.drop.threshold ? x[r] : 0.f;
       }
+      p[u] = rounded<T>(x);
     }
     if (!CLEAN) {
 #pragma unroll
@@ -387,9 +389,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kDqWaves<T,
       for (int u = 0; u < kSub; ++u) {
         Acc s{}, dp{};
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) s = mma(KV::read_row(lds[buf][0], u * 32 + (lane & 31), i, half), qf[i], s);
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) dp = mma(KV::read_row(lds[buf][1], u * 32 + (lane & 31), i, half), gf[i], dp);
+        for (int i = 0; i < kSteps; ++i) {
+          s = mma(KV::read_row(lds[buf][0], u * 32 + (lane & 31), i, half), qf[i], s);
+          dp = mma(KV::read_row(lds[buf][1], u * 32 + (lane & 31), i, half), gf[i], dp);
+        }
+        if (sizeof(T) == 2) feed<8, 2 * kSteps, 1>();
         float ds[16];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -417,12 +421,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kDqWaves<T,
         }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          Frag<T> f;
-#pragma unroll
-          for (int r = 0; r < 8; ++r) f[r] = static_cast<T>(ds[t * 8 + r]);
+          const Frag<T> f = rounded<T>(ds + t * 8);
 #pragma unroll
           for (int i = 0; i < kDT; ++i) dq[i] = mma(KV::read_columns(lds[buf][0], u * 32 + t * 16, i, lane), f, dq[i]);
         }
+        if (sizeof(T) == 2) feed<8, 2 * kDT, 2>();
       }
     }
     loads_done();
@@ -620,9 +623,7 @@ __attribute__((amdgpu_waves_per_eu(DkvShape<T, DP, DROP>::kWaves, DkvShape<T, DP
         }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          Frag<T> pf, df;
-#pragma unroll
-          for (int r = 0; r < 8; ++r) pf[r] = static_cast<T>(p[t * 8 + r]), df[r] = static_cast<T>(ds[t * 8 + r]);
+          const Frag<T> pf = rounded<T>(p + t * 8), df = rounded<T>(ds + t * 8);
 #pragma unroll
           for (int i = 0; i < kDT; ++i) {
             dv[i] = mma(QG::read_columns(lds[buf][1], sub + t * 16, i, lane), pf, dv[i]);

@@ -19,6 +19,7 @@
 #include <hip/hip_runtime.h>
 
 #include "convert.h"
+#include "counter_rng.h"
 #include "transformer_kernels.h"
 
 namespace bf_attn {
@@ -31,6 +32,16 @@ struct FragOf {
 };
 template <typename T>
 using Frag = typename FragOf<T>::type;
+
+// eight values rounded at once: two to an instruction
+template <typename T>
+__device__ __forceinline__ Frag<T> rounded(const float* x) {
+  typedef float F8 __attribute__((ext_vector_type(8)));
+  F8 f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = x[i];
+  return __builtin_convertvector(f, Frag<T>);
+}
 
 __device__ __forceinline__ Acc mma(Frag<__bf16> a, Frag<__bf16> b, Acc c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -264,15 +275,13 @@ __device__ __forceinline__ void store_row(T* row, Acc (&acc)[TILES], float f, in
       }
       const int c = dt * 32 + s * 16 + half * 8;
       if (!inside) continue;
-      T t[8], less[8];
+      const Frag<T> t = rounded<T>(x);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        t[i] = static_cast<T>(x[i]);
-        less[i] = static_cast<T>(x[i] - static_cast<float>(t[i]));
-      }
+      for (int i = 0; i < 8; ++i) x[i] -= static_cast<float>(t[i]);
+      const Frag<T> less = rounded<T>(x);
       if (c + 8 <= dim) {
-        __builtin_memcpy(row + c, t, sizeof(t));
-        if (rest) __builtin_memcpy(rest + c, less, sizeof(less));
+        __builtin_memcpy(row + c, &t, sizeof(t));
+        if (rest) __builtin_memcpy(rest + c, &less, sizeof(less));
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -347,29 +356,33 @@ __device__ __forceinline__ int sum_up_to(int x) {
   return x;
 }
 
-// Tile `number`. Causal tiles cost the more the later they are (by_cost: the
-// later, from the sequence's end, the earlier), and a long one that starts last
-// keeps the card waiting: up to 63 sequences' tiles are numbered by their cost,
-// the most expensive first. More sequences, and tiles that cost the same inside
-// one, are numbered in order.
-__device__ __forceinline__ Work find_tile(const BfAttnArgs& a, int number, int size, bool by_cost) {
+// Tile `number`. Causal tiles cost the more the later they are, and an expensive
+// one that starts last keeps the card waiting: up to 64 sequences' tiles are
+// numbered by their cost, the most expensive first, as their number from the
+// sequence's start (dk and dv: from its end). Other tiles, which cost as their
+// sequence is long, are numbered in order; sorted they took as long.
+__device__ __forceinline__ Work find_tile(const BfAttnArgs& a, int number, int size, bool causal) {
   const int lane = threadIdx.x & 63, n = a.seqs + 1;
   Work w{};
-  if (by_cost && n <= 64) {
-    const int2 b = lane < n ? bounds_of(a, lane) : make_int2(0, 0);
-    const int mine = (b.y - b.x + size - 1) / size;
-    int low = 0, high = a.rows / size + 1;  // more tiles than `number` cost `low` or more, and not `high`
-    if (wave_sum(mine) <= number) return w;
-    while (high - low > 1) {
-      const int mid = (low + high) / 2;
-      if (wave_sum(max(mine - mid, 0)) > number) low = mid;
-      else high = mid;
+  if (causal && a.seqs <= 64) {
+    const int2 b = lane < a.seqs ? bounds_of(a, lane) : make_int2(0, 0);
+    const int length = b.y - b.x, mine = (length + size - 1) / size, all = wave_sum(mine);
+    if (number >= all) {  // behind the last sequence
+      const int2 rest = bounds_of(a, a.seqs);
+      w.seq = a.seqs;
+      w.tile = number - all;
+      if (w.tile * size >= rest.y - rest.x) return w;
+    } else {
+      int low = 0, high = a.rows / size + 1;  // more tiles than `number` cost `low` or more, and not `high`
+      while (high - low > 1) {
+        const int mid = (low + high) / 2;
+        if (wave_sum(max(mine - mid, 0)) > number) low = mid;
+        else high = mid;
+      }
+      number -= wave_sum(max(mine - low - 1, 0));
+      w.seq = __ffsll(__ballot(sum_up_to(mine > low ? 1 : 0) > number)) - 1;
+      w.tile = low;
     }
-    number -= wave_sum(max(mine - low - 1, 0));
-    const bool has = mine > low;
-    const unsigned long long past = __ballot(sum_up_to(has ? 1 : 0) > number);
-    w.seq = __ffsll(past) - 1;
-    w.tile = low;
   } else {
     int first = 0, count = n, chunk = (n + 63) / 64;
     while (true) {

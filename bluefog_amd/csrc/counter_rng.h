@@ -16,13 +16,7 @@
 
 #include <cstdint>
 
-struct BfDropout {
-  const int64_t* seed_ptr;  // seed on the device, or null: `seed` holds
-  uint64_t seed;
-  uint32_t offset;
-  uint32_t threshold;  // 0: no dropout
-  float scale;
-};
+#include "transformer_kernels.h"
 
 struct BfKey {
   uint32_t k0, k1;
@@ -33,15 +27,20 @@ __device__ __forceinline__ BfKey bf_key(const BfDropout& d) {
   return {static_cast<uint32_t>(s), static_cast<uint32_t>(s >> 32)};
 }
 
+// one instruction; 0x96 is the truth table of the exclusive or of three
+__device__ __forceinline__ uint32_t bf_xor3(uint32_t a, uint32_t b, uint32_t c) {
+  return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96);
+}
+
 __device__ __forceinline__ uint4 bf_philox(uint32_t c0, uint32_t c1,
                                            uint32_t c2, uint32_t c3, BfKey k) {
 #pragma unroll
   for (int i = 0; i < 7; ++i) {
     const uint64_t a = static_cast<uint64_t>(c0) * 0xD2511F53u;
     const uint64_t b = static_cast<uint64_t>(c2) * 0xCD9E8D57u;
-    c0 = static_cast<uint32_t>(b >> 32) ^ c1 ^ k.k0;
+    c0 = bf_xor3(static_cast<uint32_t>(b >> 32), c1, k.k0);
     c1 = static_cast<uint32_t>(b);
-    c2 = static_cast<uint32_t>(a >> 32) ^ c3 ^ k.k1;
+    c2 = bf_xor3(static_cast<uint32_t>(a >> 32), c3, k.k1);
     c3 = static_cast<uint32_t>(a);
     k.k0 += 0x9E3779B9u;
     k.k1 += 0xBB67AE85u;

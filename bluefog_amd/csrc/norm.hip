@@ -16,6 +16,7 @@
 #include <hip/hip_runtime.h>
 
 #include "convert.h"
+#include "counter_rng.h"
 #include "transformer_kernels.h"
 
 namespace {

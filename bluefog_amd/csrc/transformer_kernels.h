@@ -7,7 +7,15 @@
 
 #include <hip/hip_runtime.h>
 
-#include "counter_rng.h"
+#include <cstdint>
+
+struct BfDropout {
+  const int64_t* seed_ptr;  // seed on the device, or null: `seed` holds
+  uint64_t seed;
+  uint32_t offset;
+  uint32_t threshold;  // 0: no dropout
+  float scale;
+};
 
 struct BfAttnArgs {
   const void *q, *k, *v, *dout;
