@@ -111,12 +111,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kFwdWaves<T
   // workgroup's rows. CLEAN: see below.
   const auto attend = [&](auto mode, int k0, int buf) __attribute__((always_inline)) {
     constexpr bool MASKED = decltype(mode)::value > 0, CLEAN = decltype(mode)::value > 1;
+    const int rows = KV::row_place(lane & 31, half), columns = KV::columns_place(lane);
     Acc s[kSub];
 #pragma unroll
     for (int u = 0; u < kSub; ++u) {
       s[u] = Acc{};
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) s[u] = mma(KV::read_row(lds[buf][0], u * 32 + (lane & 31), i, half), qf[i], s[u]);
+      for (int i = 0; i < kSteps; ++i) s[u] = mma(KV::read_row(lds[buf][0], rows, u * 32, i, half), qf[i], s[u]);
     }
     if (sizeof(T) == 2) feed<4, kSub * kSteps, 1>();
     if (MASKED) {
@@ -159,14 +160,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kFwdWaves<T
 #pragma unroll
       for (int u = 0; u < BN / 16; ++u)
 #pragma unroll
-        for (int i = 0; i < kDT; ++i) o[i] = mma(KV::read_columns(lds[buf][1], u * 16, i, lane), p[u], o[i]);
+        for (int i = 0; i < kDT; ++i) o[i] = mma(KV::read_columns(lds[buf][1], columns, u * 16, i), p[u], o[i]);
     } else {
 #pragma unroll
       for (int i = 0; i < kDT; ++i) {
         Acc count{};
 #pragma unroll
         for (int u = 0; u < BN / 16; ++u) {
-          Frag<T> f = KV::read_columns(lds[buf][1], u * 16, i, lane), bad, sees;
+          Frag<T> f = KV::read_columns(lds[buf][1], columns, u * 16, i), bad, sees;
 #pragma unroll
           for (int r = 0; r < 8; ++r) {
             const bool fine = fabsf(static_cast<float>(f[r])) < INFINITY;
@@ -385,13 +386,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kDqWaves<T,
     }
     if (qw < w.len && !(a.causal && k0 > qw + 31)) {
       const bool masked = k0 + BN > w.len || (a.causal && (k0 + BN - 1 > qw || qw == 0));
+      const int rows = KV::row_place(lane & 31, half), columns = KV::columns_place(lane);
 #pragma unroll
       for (int u = 0; u < kSub; ++u) {
         Acc s{}, dp{};
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
-          s = mma(KV::read_row(lds[buf][0], u * 32 + (lane & 31), i, half), qf[i], s);
-          dp = mma(KV::read_row(lds[buf][1], u * 32 + (lane & 31), i, half), gf[i], dp);
+          s = mma(KV::read_row(lds[buf][0], rows, u * 32, i, half), qf[i], s);
+          dp = mma(KV::read_row(lds[buf][1], rows, u * 32, i, half), gf[i], dp);
         }
         if (sizeof(T) == 2) feed<8, 2 * kSteps, 1>();
         float ds[16];
@@ -423,7 +425,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kDqWaves<T,
         for (int t = 0; t < 2; ++t) {
           const Frag<T> f = rounded<T>(ds + t * 8);
 #pragma unroll
-          for (int i = 0; i < kDT; ++i) dq[i] = mma(KV::read_columns(lds[buf][0], u * 32 + t * 16, i, lane), f, dq[i]);
+          for (int i = 0; i < kDT; ++i) dq[i] = mma(KV::read_columns(lds[buf][0], columns, u * 32 + t * 16, i), f, dq[i]);
         }
         if (sizeof(T) == 2) feed<8, 2 * kDT, 2>();
       }
@@ -485,6 +487,7 @@ __attribute__((amdgpu_waves_per_eu(DkvShape<T, DP, DROP>::kWaves, DkvShape<T, DP
   constexpr int BM = 32 * SPLIT * SUBS;  // queries of a step
   constexpr int kSteps = DP / 16, kDT = DP / 32;
   constexpr bool V_IN_LDS = Shape::kVInLds;
+  constexpr bool kHide = sizeof(T) == 2 && DP == 128;  // 670 TFLOP/s without, 710 with
   typedef Tile<T, BM, DP, THREADS, VEC> QG;
   typedef Tile<T, kK, DP, THREADS, VEC> Values;
   __shared__ __align__(1024) char lds[2][2][QG::kBytes];
@@ -566,14 +569,16 @@ __attribute__((amdgpu_waves_per_eu(DkvShape<T, DP, DROP>::kWaves, DkvShape<T, DP
       const int sub = (part * SUBS + n32) * 32, iw = i0 + sub;  // the wave's queries
       if (jw < w.len && iw < w.len && !(a.causal && iw + 31 < jw)) {
         const bool masked = iw + 32 > w.len || (a.causal && (iw < jw + 31 || iw == 0)) || w.len == 1;
+        const int rows = here<kHide>(QG::row_place(lane & 31, half)), columns = here<kHide>(QG::columns_place(lane));
+        const int own = here<kHide>(Values::row_place(jl, half));
         Acc s{}, dp{};
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) s = mma(QG::read_row(lds[buf][0], sub + (lane & 31), i, half), kf[i], s);
+        for (int i = 0; i < kSteps; ++i) s = mma(QG::read_row(lds[buf][0], rows, sub, i, half), kf[i], s);
 #pragma unroll
         for (int i = 0; i < kSteps; ++i)
-          dp = mma(QG::read_row(lds[buf][1], sub + (lane & 31), i, half),
-                   V_IN_LDS ? Values::read_row(v_lds, jl, i, half) : vf[V_IN_LDS ? 0 : i], dp);
-        if (sizeof(T) == 2) feed<V_IN_LDS ? 8 : 6, 2 * kSteps, V_IN_LDS ? 2 : 1>();
+          dp = mma(QG::read_row(lds[buf][1], rows, sub, i, half),
+                   V_IN_LDS ? Values::read_row(v_lds, own, 0, i, half) : vf[V_IN_LDS ? 0 : i], dp);
+        if (sizeof(T) == 2) feed<6, 2 * kSteps, 2>();
         if (DROP) {
           // the lane's share of a query's mask, as the forward pass has it
           uint32_t bits = 0;
@@ -626,8 +631,8 @@ __attribute__((amdgpu_waves_per_eu(DkvShape<T, DP, DROP>::kWaves, DkvShape<T, DP
           const Frag<T> pf = rounded<T>(p + t * 8), df = rounded<T>(ds + t * 8);
 #pragma unroll
           for (int i = 0; i < kDT; ++i) {
-            dv[i] = mma(QG::read_columns(lds[buf][1], sub + t * 16, i, lane), pf, dv[i]);
-            dk[i] = mma(QG::read_columns(lds[buf][0], sub + t * 16, i, lane), df, dk[i]);
+            dv[i] = mma(QG::read_columns(lds[buf][1], columns, sub + t * 16, i), pf, dv[i]);
+            dk[i] = mma(QG::read_columns(lds[buf][0], columns, sub + t * 16, i), df, dk[i]);
           }
         }
         if (sizeof(T) == 2) feed<8, 4 * kDT, 2>();
@@ -673,10 +678,12 @@ __global__ __launch_bounds__(256) void attn_fold_k(T* first, T* second, const fl
     if (u < n) out[u] = static_cast<T>(sum[u]);
 }
 
+constexpr long kMostGroups = 0xFFFFFF;  // of 256 threads: a launch has less than 2^32
+
 template <typename T>
 hipError_t fold(void* first, void* second, const float* partial, long all, int slices, hipStream_t stream) {
   const long blocks = (all + 1023) / 1024;
-  if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
+  if (blocks > kMostGroups) return hipErrorInvalidValue;
   hipLaunchKernelGGL(attn_fold_k<T>, dim3(blocks, second ? 2 : 1), dim3(256), 0, stream, static_cast<T*>(first),
                      static_cast<T*>(second), partial, all, slices);
   return hipGetLastError();
@@ -685,13 +692,13 @@ hipError_t fold(void* first, void* second, const float* partial, long all, int s
 template <typename T, int DP, bool VEC>
 hipError_t fwd(const BfAttnArgs& a, hipStream_t stream) {
   const long groups = units(most_tiles(a, 128) * a.key_slices, a.heads);
-  if (groups > 0x7FFFFFFF) return hipErrorInvalidValue;
+  if (groups > kMostGroups) return hipErrorInvalidValue;
   if (a.drop.threshold) hipLaunchKernelGGL((attn_fwd_k<T, DP, VEC, true>), dim3(groups), dim3(256), 0, stream, a);
   else hipLaunchKernelGGL((attn_fwd_k<T, DP, VEC, false>), dim3(groups), dim3(256), 0, stream, a);
   if (hipError_t e = hipGetLastError()) return e;
   if (a.key_slices == 1) return hipSuccess;
   const long blocks = (static_cast<long>(a.rows) * a.heads * ((a.dim + 3) / 4) + 255) / 256;
-  if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
+  if (blocks > kMostGroups) return hipErrorInvalidValue;
   hipLaunchKernelGGL(attn_join_k<T>, dim3(blocks), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
@@ -706,7 +713,7 @@ template <typename T, int DP, bool VEC, bool DROP>
 hipError_t bwd(const BfAttnArgs& a, bool need_dkv, hipStream_t stream) {
   const long groups = units(most_tiles(a, 128) * a.key_slices, a.heads);
   const long shared = units(most_tiles(a, 128) * a.query_slices, a.kv_heads);
-  if (groups > 0x7FFFFFFF || shared > 0x7FFFFFFF) return hipErrorInvalidValue;
+  if (groups > kMostGroups || shared > kMostGroups / 2) return hipErrorInvalidValue;
   hipLaunchKernelGGL((attn_dq_k<T, DP, VEC, DROP>), dim3(groups), dim3(256), 0, stream, a);
   if (hipError_t e = hipGetLastError()) return e;
   if (a.key_slices > 1)

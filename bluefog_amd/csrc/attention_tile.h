@@ -101,39 +101,48 @@ struct Tile {
     for (int i = threadIdx.x * 16; i < bytes; i += THREADS * 16) *reinterpret_cast<uint4*>(lds + i) = uint4{0, 0, 0, 0};
   }
 
-  // fragment of row `row`, inner positions = columns of step `step`
-  static __device__ __forceinline__ Frag<T> read_row(const char* lds, int row, int step, int half) {
+  // Places of a lane in a tile, from which those of its fragments differ in bits
+  // of the chunk: row_place for row `row` (columns of step 0), columns_place for
+  // column `lane & 31` (rows 0 and on). For f32 they are row and lane themselves.
+  static __device__ __forceinline__ int row_place(int row, int half) {
+    return sizeof(T) == 2 ? at(row, half) : row;
+  }
+  static __device__ __forceinline__ int columns_place(int lane) {
+    if (sizeof(T) == 4) return lane;
+    // sixteen lanes give the addresses of 4 rows of 16 values, four to a lane
+    return at(4 * (lane >> 5) + ((lane & 15) >> 2), ((lane & 16) >> 3) + ((lane & 3) >> 1)) + (lane & 1) * 8;
+  }
+
+  // fragment of the place's row, `down` (a multiple of 16) rows on, inner
+  // positions = columns of step `step`
+  static __device__ __forceinline__ Frag<T> read_row(const char* lds, int place, int down, int step, int half) {
     Frag<T> f;
     if constexpr (sizeof(T) == 2) {
-      f = *reinterpret_cast<const Frag<T>*>(lds + at(row, step * 2 + half));
+      f = *reinterpret_cast<const Frag<T>*>(lds + (place ^ (step << 5)) + down * kRowBytes);
     } else {
       typedef float F4 __attribute__((ext_vector_type(4)));
-      const F4 x = *reinterpret_cast<const F4*>(lds + at(row, step * 4 + half * 2));
-      const F4 y = *reinterpret_cast<const F4*>(lds + at(row, step * 4 + half * 2 + 1));
+      const F4 x = *reinterpret_cast<const F4*>(lds + at(place + down, step * 4 + half * 2));
+      const F4 y = *reinterpret_cast<const F4*>(lds + at(place + down, step * 4 + half * 2 + 1));
       f = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
     }
     return f;
   }
 
-  // fragment of column 32 * dt + (lane & 31), inner positions = rows
-  // base + {4 half .. + 3, 8 + 4 half .. + 3}
-  static __device__ __forceinline__ Frag<T> read_columns(const char* lds, int base, int dt, int lane) {
-    const int half = lane >> 5;
+  // fragment of the place's column, 32 * dt columns on, inner positions = rows
+  // base (a multiple of 16) + {4 half .. + 3, 8 + 4 half .. + 3}
+  static __device__ __forceinline__ Frag<T> read_columns(const char* lds, int place, int base, int dt) {
     Frag<T> f;
     if constexpr (sizeof(T) == 2) {
-      // the transposing read: sixteen lanes give the addresses of 4 rows of 16
-      // values, four to a lane, and lane i gets column i of the four rows
+      // the transposing read: lane i of sixteen gets column i of the four rows
       typedef short S4 __attribute__((ext_vector_type(4)));
-      const int row = base + 4 * half + ((lane & 15) >> 2);
-      const int c = dt * 32 + (lane & 16) + (lane & 3) * 4;
       S4 part[2];
 #pragma unroll
       for (int k = 0; k < 2; ++k)
         part[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) S4*)(lds + at(row + 8 * k, c / 8) + (c % 8) * 2));
+            (__attribute__((address_space(3))) S4*)(lds + (place ^ (dt << 6) ^ (k << 4)) + (base + 8 * k) * kRowBytes));
       __builtin_memcpy(&f, part, sizeof(f));
     } else {
-      const int c = dt * 32 + (lane & 31);
+      const int c = dt * 32 + (place & 31), half = place >> 5;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         f[j] = *reinterpret_cast<const T*>(lds + at(base + row_of(j, half), c / kEach) + (c % kEach) * sizeof(T));
@@ -236,6 +245,15 @@ __device__ __forceinline__ void weave() {
     __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
     if (VALU) __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
   }
+}
+
+// A place as something that the compiler cannot work out ahead: the fragments'
+// addresses are then made where they are used, one instruction each, in place of
+// a register each over the whole loop.
+template <bool HIDE>
+__device__ __forceinline__ int here(int place) {
+  if (HIDE) asm volatile("" : "+v"(place));
+  return place;
 }
 
 // fragment of a row in memory, columns of step `step`; 0 behind dim
@@ -414,6 +432,6 @@ __device__ __forceinline__ Work find_tile(const BfAttnArgs& a, int number, int s
 }
 
 // tiles of `size` rows that any bounds can have, the rows behind included
-inline long most_tiles(const BfAttnArgs& a, int size) { return a.rows / size + a.seqs + 1; }
+inline long most_tiles(const BfAttnArgs& a, int size) { return a.rows / size + static_cast<long>(a.seqs) + 1; }
 
 }  // namespace bf_attn

@@ -365,85 +365,87 @@ __device__ __forceinline__ void join8(const BfNormArgs& a, long row, int c, BfKe
   else join8<false>(a, row, c, key, x, r, z, kept);
 }
 
-constexpr int kWideWaves = 16;
-
-template <typename TX, typename TR>
-__global__ __launch_bounds__(kWideWaves * 64) void norm_fwd_wide_k(BfNormArgs a) {
-  __shared__ float lds[kWideWaves];
+template <typename TX, typename TR, int WAVES>
+__global__ __launch_bounds__(threads_of(WAVES)) void norm_fwd_wide_k(BfNormArgs a) {
+  __shared__ float lds[WAVES];
+  constexpr int kLanes = WAVES * 64, kStep = kLanes * kVec;
   const BfKey key = a.drop.threshold ? bf_key(a.drop) : BfKey{0, 0};
-  const float width = static_cast<float>(a.width);  // divided by: a constant row has exactly its mean
-  const long row = blockIdx.x;
-  const int first = threadIdx.x * kVec;
-  constexpr int kStep = kWideWaves * 64 * kVec;
-  float s = 0.f, q = 0.f, z[kVec];
-  bool kept[kVec];
-  for (int c = first; c < a.width; c += kStep) {
-    join8<TX, TR>(a, row, c, key, z, kept);
+  const float width = static_cast<float>(a.width);
+  const int first = threadIdx.x % kLanes * kVec;
+  const long step = static_cast<long>(gridDim.x) * rows_of(WAVES);
+  for (long row = static_cast<long>(blockIdx.x) * rows_of(WAVES) + threadIdx.x / kLanes; row < a.rows; row += step) {
+    float s = 0.f, q = 0.f, z[kVec];
+    bool kept[kVec];
+    for (int c = first; c < a.width; c += kStep) {
+      join8<TX, TR>(a, row, c, key, z, kept);
 #pragma unroll
-    for (int u = 0; u < kVec; ++u) s += c + u < a.width ? z[u] : 0.f;
-  }
-  const float mean = row_sum<kWideWaves>(s, lds) / width;
-  for (int c = first; c < a.width; c += kStep) {
-    join8<TX, TR>(a, row, c, key, z, kept);
+      for (int u = 0; u < kVec; ++u) s += c + u < a.width ? z[u] : 0.f;
+    }
+    const float mean = row_sum<WAVES>(s, lds) / width;
+    for (int c = first; c < a.width; c += kStep) {
+      join8<TX, TR>(a, row, c, key, z, kept);
 #pragma unroll
-    for (int u = 0; u < kVec; ++u) q += c + u < a.width ? (z[u] - mean) * (z[u] - mean) : 0.f;
-  }
-  const float rstd = 1.f / sqrtf(row_sum<kWideWaves>(q, lds) / width + a.eps);
-  if (a.mean && threadIdx.x == 0) {
-    a.mean[row] = mean;
-    a.rstd[row] = rstd;
-  }
-  for (int c = first; c < a.width; c += kStep) {
-    const int n = a.width - c;
-    float w[kVec], b[kVec];
-    join8<TX, TR>(a, row, c, key, z, kept);
-    load8_param<TX>(a.weight, c, n, a.weight_f32, 1.f, w);
-    load8_param<TX>(a.bias, c, n, a.weight_f32, 0.f, b);
+      for (int u = 0; u < kVec; ++u) q += c + u < a.width ? (z[u] - mean) * (z[u] - mean) : 0.f;
+    }
+    const float rstd = 1.f / sqrtf(row_sum<WAVES>(q, lds) / width + a.eps);
+    if (a.mean && threadIdx.x % kLanes == 0) {
+      a.mean[row] = mean;
+      a.rstd[row] = rstd;
+    }
+    for (int c = first; c < a.width; c += kStep) {
+      const int n = a.width - c;
+      float w[kVec], b[kVec];
+      join8<TX, TR>(a, row, c, key, z, kept);
+      load8_param<TX>(a.weight, c, n, a.weight_f32, 1.f, w);
+      load8_param<TX>(a.bias, c, n, a.weight_f32, 0.f, b);
 #pragma unroll
-    for (int u = 0; u < kVec; ++u) b[u] += (z[u] - mean) * rstd * w[u];
-    store8(static_cast<TR*>(a.y) + row * a.width + c, n, b);
+      for (int u = 0; u < kVec; ++u) b[u] += (z[u] - mean) * rstd * w[u];
+      store8(static_cast<TR*>(a.y) + row * a.width + c, n, b);
+    }
   }
 }
 
-template <typename TX, typename TR>
-__global__ __launch_bounds__(kWideWaves * 64) void norm_bwd_wide_k(BfNormArgs a) {
-  __shared__ float2 lds[kWideWaves];
+template <typename TX, typename TR, int WAVES>
+__global__ __launch_bounds__(threads_of(WAVES)) void norm_bwd_wide_k(BfNormArgs a) {
+  __shared__ float2 lds[WAVES];
+  constexpr int kLanes = WAVES * 64, kStep = kLanes * kVec;
   const BfKey key = a.drop.threshold ? bf_key(a.drop) : BfKey{0, 0};
-  const float width = static_cast<float>(a.width);  // divided by: a constant row has exactly its mean
-  const long row = blockIdx.x;
-  const float mean = a.mean[row], rstd = a.rstd[row];
-  const int first = threadIdx.x * kVec;
-  constexpr int kStep = kWideWaves * 64 * kVec;
-  float s = 0.f, q = 0.f, z[kVec], g[kVec], w[kVec];
-  bool kept[kVec];
-  for (int c = first; c < a.width; c += kStep) {
-    const int n = a.width - c;
-    join8<TX, TR>(a, row, c, key, z, kept);
-    load8(static_cast<const TR*>(a.dy) + row * a.dy_row + c, n, g);
-    load8_param<TX>(a.weight, c, n, a.weight_f32, 1.f, w);
+  const float width = static_cast<float>(a.width);
+  const int first = threadIdx.x % kLanes * kVec;
+  const long step = static_cast<long>(gridDim.x) * rows_of(WAVES);
+  for (long row = static_cast<long>(blockIdx.x) * rows_of(WAVES) + threadIdx.x / kLanes; row < a.rows; row += step) {
+    const float mean = a.mean[row], rstd = a.rstd[row];
+    float s = 0.f, q = 0.f, z[kVec], g[kVec], w[kVec];
+    bool kept[kVec];
+    for (int c = first; c < a.width; c += kStep) {
+      const int n = a.width - c;
+      join8<TX, TR>(a, row, c, key, z, kept);
+      load8(static_cast<const TR*>(a.dy) + row * a.dy_row + c, n, g);
+      load8_param<TX>(a.weight, c, n, a.weight_f32, 1.f, w);
 #pragma unroll
-    for (int u = 0; u < kVec; ++u) {
-      const float t = u < n ? g[u] * w[u] : 0.f;
-      s += t;
-      q += u < n ? t * (z[u] - mean) * rstd : 0.f;
+      for (int u = 0; u < kVec; ++u) {
+        const float t = u < n ? g[u] * w[u] : 0.f;
+        s += t;
+        q += u < n ? t * (z[u] - mean) * rstd : 0.f;
+      }
     }
-  }
-  const float2 sums = row_sum2<kWideWaves>(s, q, lds);
-  const float m1 = sums.x / width, m2 = sums.y / width;
-  for (int c = first; c < a.width; c += kStep) {
-    const int n = a.width - c;
-    join8<TX, TR>(a, row, c, key, z, kept);
-    load8(static_cast<const TR*>(a.dy) + row * a.dy_row + c, n, g);
-    load8_param<TX>(a.weight, c, n, a.weight_f32, 1.f, w);
+    const float2 sums = row_sum2<WAVES>(s, q, lds);
+    const float m1 = sums.x / width, m2 = sums.y / width;
+    for (int c = first; c < a.width; c += kStep) {
+      const int n = a.width - c;
+      join8<TX, TR>(a, row, c, key, z, kept);
+      load8(static_cast<const TR*>(a.dy) + row * a.dy_row + c, n, g);
+      load8_param<TX>(a.weight, c, n, a.weight_f32, 1.f, w);
 #pragma unroll
-    for (int u = 0; u < kVec; ++u) g[u] = rstd * (g[u] * w[u] - m1 - (z[u] - mean) * rstd * m2);
-    if (a.dr) store8(static_cast<TR*>(a.dr) + row * a.width + c, n, g);
-    if (!a.dx) continue;
-    if (a.drop.threshold) {
+      for (int u = 0; u < kVec; ++u) g[u] = rstd * (g[u] * w[u] - m1 - (z[u] - mean) * rstd * m2);
+      if (a.dr) store8(static_cast<TR*>(a.dr) + row * a.width + c, n, g);
+      if (!a.dx) continue;
+      if (a.drop.threshold) {
 #pragma unroll
-      for (int u = 0; u < kVec; ++u) g[u] = kept[u] ? g[u] * a.drop.scale : 0.f;
+        for (int u = 0; u < kVec; ++u) g[u] = kept[u] ? g[u] * a.drop.scale : 0.f;
+      }
+      store8(static_cast<TX*>(a.dx) + row * a.width + c, n, g);
     }
-    store8(static_cast<TX*>(a.dx) + row * a.width + c, n, g);
   }
 }
 
@@ -522,7 +524,6 @@ __global__ __launch_bounds__(256) void dropout_k(T* __restrict__ y, const T* __r
 // ---------------------------------------------------------------------------
 
 constexpr int kWidest = 16384;
-constexpr int kWideSlots = 64;
 
 bool in_registers(int width) { return width >= kVec && width <= kWidest; }
 
@@ -534,7 +535,10 @@ long filling(int waves, int deep) { return 256L * 4 * deep / (threads_of(waves) 
 
 // workgroups of the backward pass: each leaves 8 * width bytes of partial sums
 int slots_of(long rows, int width) {
-  if (!in_registers(width)) return static_cast<int>(rows < kWideSlots ? rows : kWideSlots);
+  if (!in_registers(width)) {
+    const long most = width < kVec ? 1024 : 64;  // a slot of few columns is a small thing
+    return static_cast<int>(rows < most ? rows : most);
+  }
   const int waves = waves_of(width);
   const long groups = (rows + rows_of(waves) - 1) / rows_of(waves), most = filling(waves, 4);
   return static_cast<int>(groups < most ? groups : most);
@@ -572,14 +576,12 @@ void launch(bool backward, const BfNormArgs& a, long grid, hipStream_t stream) {
 struct Fwd {
   template <typename TX, typename TR>
   static hipError_t run(const BfNormArgs& a, hipStream_t stream) {
-    if (a.rows > 0x7FFFFFFF) return hipErrorInvalidValue;
-    if (!in_registers(a.width)) {
-      hipLaunchKernelGGL((norm_fwd_wide_k<TX, TR>), dim3(a.rows), dim3(kWideWaves * 64), 0, stream, a);
-    } else {
-      const int waves = waves_of(a.width);
-      const long groups = (a.rows + rows_of(waves) - 1) / rows_of(waves), most = filling(waves, 8);
-      launch<TX, TR>(false, a, groups < most ? groups : most, stream);
-    }
+    const int waves = waves_of(a.width);
+    const long groups = (a.rows + rows_of(waves) - 1) / rows_of(waves), most = filling(waves, 8);
+    const long grid = groups < most ? groups : most;
+    if (in_registers(a.width)) launch<TX, TR>(false, a, grid, stream);
+    else if (waves == 1) hipLaunchKernelGGL((norm_fwd_wide_k<TX, TR, 1>), dim3(grid), dim3(threads_of(1)), 0, stream, a);
+    else hipLaunchKernelGGL((norm_fwd_wide_k<TX, TR, 16>), dim3(grid), dim3(threads_of(16)), 0, stream, a);
     return hipGetLastError();
   }
 };
@@ -587,11 +589,13 @@ struct Fwd {
 struct Bwd {
   template <typename TX, typename TR>
   static hipError_t run(const BfNormArgs& a, hipStream_t stream) {
-    if (a.rows > 0x7FFFFFFF) return hipErrorInvalidValue;
-    const int slots = slots_of(a.rows, a.width);
+    const int slots = slots_of(a.rows, a.width), waves = waves_of(a.width);
     if (!in_registers(a.width)) {
       if (a.dx || a.dr) {
-        hipLaunchKernelGGL((norm_bwd_wide_k<TX, TR>), dim3(a.rows), dim3(kWideWaves * 64), 0, stream, a);
+        const long groups = (a.rows + rows_of(waves) - 1) / rows_of(waves), most = filling(waves, 8);
+        const long grid = groups < most ? groups : most;
+        if (waves == 1) hipLaunchKernelGGL((norm_bwd_wide_k<TX, TR, 1>), dim3(grid), dim3(threads_of(1)), 0, stream, a);
+        else hipLaunchKernelGGL((norm_bwd_wide_k<TX, TR, 16>), dim3(grid), dim3(threads_of(16)), 0, stream, a);
         if (hipError_t e = hipGetLastError()) return e;
       }
       if (a.partial)
@@ -622,7 +626,7 @@ hipError_t dispatch(const BfNormArgs& a, int x_dtype, int r_dtype, hipStream_t s
 template <typename T>
 hipError_t drop(void* y, const void* x, long n, const BfDropout& d, hipStream_t stream) {
   const long blocks = (n + 256 * kVec - 1) / (256 * kVec);
-  if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
+  if (blocks > 0xFFFFFF) return hipErrorInvalidValue;  // a launch has less than 2^32 threads
   hipLaunchKernelGGL(dropout_k<T>, dim3(blocks), dim3(256), 0, stream, static_cast<T*>(y), static_cast<const T*>(x), n,
                      d);
   return hipGetLastError();

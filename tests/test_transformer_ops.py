@@ -226,6 +226,7 @@ def attention_agrees(device, dtype, lengths, heads=2, kv_heads=1, dim=64, causal
 
 
 LENGTHS = [
+    (3,) * 70, (40, 0, 1) * 40, (1,) * 300,  # more sequences than lanes
     (1,), (2,), (1, 1, 1), (17,), (31, 33), (0, 5, 0, 0, 64, 0), (127, 1, 129), (200, 3), (65, 63, 2, 130),
 ]
 
@@ -396,6 +397,24 @@ def test_attention_gradient_of_a_sum(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_attention_twice_through_one_graph(device):
+    """A kept graph gives the same gradients again; a wide batch of thousands
+    of sequences is found row by row."""
+    q, k, v, dout = attention_inputs((33, 7), 4, 2, 64, torch.bfloat16, device)
+    out = bf.packed_attention(q, k, v, ends_of((33, 7), device), causal=True, dropout_p=0.1, seed=5)
+    first = torch.autograd.grad(out, (q, k, v), dout, retain_graph=True)
+    for a, b in zip(first, torch.autograd.grad(out, (q, k, v), dout)):
+        assert torch.equal(a, b)
+    lengths = [n % 3 for n in range(5000)]
+    x = torch.randn(sum(lengths), 1, 8, device=device)
+    ones = bf.packed_attention(torch.zeros_like(x), x, x, ends_of(lengths, device))
+    # equal scores: the mean of a sequence's rows (its one or two), exactly
+    row = torch.arange(len(x), device=device)
+    pair = torch.where(row % 3 == 0, row, torch.where(row % 3 == 1, row + 1, row - 1))
+    assert torch.allclose(ones, (x + x[pair.clamp_max(len(x) - 1)]) / 2, rtol=0, atol=2.0 ** -22)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_attention_nothing_to_do(device):
     cu0, cu = ends_of((), device), ends_of((0, 0), device)
     for c in (cu0, cu):
@@ -537,6 +556,13 @@ def test_norm_widths(device, dtype, width):
 def test_norm_rows(device, dtype, rows):
     norm_agrees(device, dtype, (rows, 96), residual=dtype, seed=rows)
     norm_agrees(device, dtype, (rows, 130), bias=False, seed=rows)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("width", [1, 3, 5, 7])
+def test_norm_narrow_rows(device, width):
+    norm_agrees(device, torch.float32, (40000, width), residual=torch.float32, p=0.1, seed=width)
+    norm_agrees(device, torch.bfloat16, (700, width), weights=torch.bfloat16, seed=width)
 
 
 @pytest.mark.parametrize("device", DEVICES)
