@@ -107,28 +107,29 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kFwdWaves<T
   const BfKey key = DROP ? bf_key(a.drop) : BfKey{0, 0};
   const float c = a.scale * kLog2e;
   float m = -INFINITY, l = 0.f;  // of scores without c
-  // One tile of keys. MASKED: some of them are not seen by some of the
-  // workgroup's rows. CLEAN: see below.
-  const auto attend = [&](auto mode, int k0, int buf) __attribute__((always_inline)) {
+  // One tile of keys, the first 32 * SUBS of them. MASKED: some of them are not
+  // seen by some of the workgroup's rows. CLEAN: see below.
+  const auto attend = [&](auto mode, auto subs, int k0, int buf) __attribute__((always_inline)) {
     constexpr bool MASKED = decltype(mode)::value > 0, CLEAN = decltype(mode)::value > 1;
+    constexpr int SUBS = decltype(subs)::value;
     const int rows = KV::row_place(lane & 31, half), columns = KV::columns_place(lane);
-    Acc s[kSub];
+    Acc s[SUBS];
 #pragma unroll
-    for (int u = 0; u < kSub; ++u) {
+    for (int u = 0; u < SUBS; ++u) {
       s[u] = Acc{};
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) s[u] = mma(KV::read_row(lds[buf][0], rows, u * 32, i, half), qf[i], s[u]);
     }
-    if (sizeof(T) == 2) feed<4, kSub * kSteps, 1>();
+    if (sizeof(T) == 2) feed<4, SUBS * kSteps, 1>();
     if (MASKED) {
 #pragma unroll
-      for (int u = 0; u < kSub; ++u)
+      for (int u = 0; u < SUBS; ++u)
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[u][r] = k0 + u * 32 + row_of(r, half) < seen ? s[u][r] : -INFINITY;
     }
     float top = s[0][0];
 #pragma unroll
-    for (int u = 0; u < kSub; ++u)
+    for (int u = 0; u < SUBS; ++u)
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
     top = fmaxf(top, swap_halves(top));
@@ -142,9 +143,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kFwdWaves<T
       m = grown;
     }
     const float base = m == -INFINITY ? 0.f : m * c;  // all scores so far -inf: P = 0
-    Frag<T> p[BN / 16];
+    Frag<T> p[2 * SUBS];
 #pragma unroll
-    for (int u = 0; u < BN / 16; ++u) {
+    for (int u = 0; u < 2 * SUBS; ++u) {
       uint4 bits;
       if (DROP) bits = bf_philox((k0 / 16 + u) * 2 + half, static_cast<uint32_t>(row), h, a.drop.offset, key);
       float x[8];
@@ -158,7 +159,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kFwdWaves<T
     }
     if (!CLEAN) {
 #pragma unroll
-      for (int u = 0; u < BN / 16; ++u)
+      for (int u = 0; u < 2 * SUBS; ++u)
 #pragma unroll
         for (int i = 0; i < kDT; ++i) o[i] = mma(KV::read_columns(lds[buf][1], columns, u * 16, i), p[u], o[i]);
     } else {
@@ -166,7 +167,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kFwdWaves<T
       for (int i = 0; i < kDT; ++i) {
         Acc count{};
 #pragma unroll
-        for (int u = 0; u < BN / 16; ++u) {
+        for (int u = 0; u < 2 * SUBS; ++u) {
           Frag<T> f = KV::read_columns(lds[buf][1], columns, u * 16, i), bad, sees;
 #pragma unroll
           for (int r = 0; r < 8; ++r) {
@@ -196,12 +197,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kFwdWaves<T
     };
     for (; k0 < whole; k0 += BN, buf ^= 1) {
       next();
-      if (qw < w.len) attend(Mode<0>(), k0, buf);
+      if (qw < w.len) attend(Mode<0>(), Mode<kSub>(), k0, buf);
       loads_done();
     }
     for (; k0 < range.y; k0 += BN, buf ^= 1) {
       next();
-      if (qw < w.len && !(a.causal && k0 > qw + 31)) attend(masked, k0, buf);
+      const int seen_here = min(range.y, a.causal ? qw + 32 : w.len) - k0;  // keys that some row of the wave sees
+      if (qw < w.len && seen_here > 0) {
+        if (kSub == 1 || seen_here > 32) attend(masked, Mode<kSub>(), k0, buf);
+        else attend(masked, Mode<1>(), k0, buf);
+      }
       loads_done();
     }
   };
@@ -389,6 +394,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kDqWaves<T,
       const int rows = KV::row_place(lane & 31, half), columns = KV::columns_place(lane);
 #pragma unroll
       for (int u = 0; u < kSub; ++u) {
+        if (u && masked && k0 + u * 32 >= (a.causal ? min(w.len, qw + 32) : w.len)) continue;  // none sees them
         Acc s{}, dp{};
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {

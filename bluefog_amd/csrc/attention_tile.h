@@ -380,50 +380,53 @@ __device__ __forceinline__ int sum_up_to(int x) {
 // sequence's start (dk and dv: from its end). Other tiles, which cost as their
 // sequence is long, are numbered in order; sorted they took as long.
 __device__ __forceinline__ Work find_tile(const BfAttnArgs& a, int number, int size, bool causal) {
-  const int lane = threadIdx.x & 63, n = a.seqs + 1;
+  const int lane = threadIdx.x & 63;
   Work w{};
-  if (causal && a.seqs <= 64) {
-    const int2 b = lane < a.seqs ? bounds_of(a, lane) : make_int2(0, 0);
-    const int length = b.y - b.x, mine = (length + size - 1) / size, all = wave_sum(mine);
-    if (number >= all) {  // behind the last sequence
-      const int2 rest = bounds_of(a, a.seqs);
-      w.seq = a.seqs;
-      w.tile = number - all;
-      if (w.tile * size >= rest.y - rest.x) return w;
-    } else {
-      int low = 0, high = a.rows / size + 1;  // more tiles than `number` cost `low` or more, and not `high`
-      while (high - low > 1) {
-        const int mid = (low + high) / 2;
-        if (wave_sum(max(mine - mid, 0)) > number) low = mid;
-        else high = mid;
-      }
-      number -= wave_sum(max(mine - low - 1, 0));
-      w.seq = __ffsll(__ballot(sum_up_to(mine > low ? 1 : 0) > number)) - 1;
-      w.tile = low;
-    }
-  } else {
-    int first = 0, count = n, chunk = (n + 63) / 64;
-    while (true) {
-      int mine = 0;
+  int first = 0, count = a.seqs, chunk = (a.seqs + 63) / 64, mine = 0;
+  const auto tiles_of = [&]() __attribute__((always_inline)) {  // of the lane's `chunk` sequences
+    int sum = 0;
 #pragma unroll 8
-      for (int i = 0; i < chunk; ++i) {  // unguarded, so that the loads go out together
-        const int at = lane * chunk + i;
-        const int2 b = bounds_of(a, first + min(at, count - 1));
-        mine += at < count ? (b.y - b.x + size - 1) / size : 0;
-      }
-      const int upto = sum_up_to(mine);
-      const unsigned long long past = __ballot(upto > number);
-      if (!past) return w;
-      const int pick = __ffsll(past) - 1;
-      number -= __shfl(upto - mine, pick, 64);
+    for (int i = 0; i < chunk; ++i) {  // unguarded, so that the loads go out together
+      const int at = lane * chunk + i;
+      const int2 b = bounds_of(a, first + min(at, count - 1));
+      sum += at < count ? (b.y - b.x + size - 1) / size : 0;
+    }
+    return sum;
+  };
+  if (count) mine = tiles_of();
+  int upto = sum_up_to(mine);
+  const int all = __builtin_amdgcn_readlane(upto, 63);
+  if (number >= all) {  // behind the last sequence
+    const int2 rest = bounds_of(a, a.seqs);
+    w.seq = a.seqs;
+    w.tile = number - all;
+    if (w.tile * size >= rest.y - rest.x) return w;
+  } else if (causal && chunk == 1) {
+    int low = 0, high = a.rows / size + 1;  // more tiles than `number` cost `low` or more, and not `high`
+    while (high - low > 1) {
+      const int mid = (low + high) / 2;
+      if (wave_sum(max(mine - mid, 0)) > number) low = mid;
+      else high = mid;
+    }
+    number -= wave_sum(max(mine - low - 1, 0));
+    w.seq = __ffsll(__ballot(sum_up_to(mine > low ? 1 : 0) > number)) - 1;
+    w.tile = low;
+  } else {
+    while (true) {
+      const int pick = __ffsll(__ballot(upto > number)) - 1;
+      number -= __builtin_amdgcn_readlane(upto - mine, pick);
       first += pick * chunk;
       if (chunk == 1) break;
       count = min(chunk, count - pick * chunk);
       chunk = (count + 63) / 64;
+      mine = tiles_of();
+      upto = sum_up_to(mine);
     }
-    w.seq = __builtin_amdgcn_readfirstlane(first);
-    w.tile = __builtin_amdgcn_readfirstlane(number);
+    w.seq = first;
+    w.tile = number;
   }
+  w.seq = __builtin_amdgcn_readfirstlane(w.seq);
+  w.tile = __builtin_amdgcn_readfirstlane(w.tile);
   const int2 b = bounds_of(a, w.seq);
   w.begin = b.x;
   w.len = b.y - b.x;
