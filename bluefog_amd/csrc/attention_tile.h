@@ -43,6 +43,15 @@ __device__ __forceinline__ Frag<T> rounded(const float* x) {
   return __builtin_convertvector(f, Frag<T>);
 }
 
+// and what that took from them
+template <typename T>
+__device__ __forceinline__ Frag<T> rest_of(const float* x, Frag<T> of) {
+  float less[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) less[i] = x[i] - static_cast<float>(of[i]);
+  return rounded<T>(less);
+}
+
 __device__ __forceinline__ Acc mma(Frag<__bf16> a, Frag<__bf16> b, Acc c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
@@ -293,10 +302,7 @@ __device__ __forceinline__ void store_row(T* row, Acc (&acc)[TILES], float f, in
       }
       const int c = dt * 32 + s * 16 + half * 8;
       if (!inside) continue;
-      const Frag<T> t = rounded<T>(x);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] -= static_cast<float>(t[i]);
-      const Frag<T> less = rounded<T>(x);
+      const Frag<T> t = rounded<T>(x), less = rest_of<T>(x, t);
       if (c + 8 <= dim) {
         __builtin_memcpy(row + c, &t, sizeof(t));
         if (rest) __builtin_memcpy(rest + c, &less, sizeof(less));
