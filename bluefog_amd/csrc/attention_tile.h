@@ -198,7 +198,7 @@ struct Loader {
           for (int n = 0; n < kLoads; ++n)
             load_to_lds<16>(from + static_cast<uint64_t>(step) * (n * kRound) + at, lds + n * THREADS * 16 + wave * 1024);
       } else {
-        const uint32_t most = (last - first) * step;
+        const uint32_t most = min(last - first, ROWS - 1) * step;
         uint32_t off = threadIdx.x * 16;
         asm volatile("" : "+v"(off));  // worked out here: kept over the loop, it would cost the loop registers
 #pragma unroll
@@ -210,7 +210,7 @@ struct Loader {
       }
     } else {
       // rows that do not start on 16 bytes: through registers, unaligned
-      const uint32_t most = (last - first) * step;
+      const uint32_t most = min(last - first, ROWS - 1) * step;
 #pragma unroll 4
       for (uint32_t off = threadIdx.x * 16; off < Of::kBytes; off += THREADS * 16) {
         const int r = off / Of::kRowBytes, c = (off % Of::kRowBytes >> 4) * Of::kEach;
@@ -243,16 +243,6 @@ __device__ __forceinline__ void feed() {
   for (int i = 0; i < PRODUCTS; ++i) {
     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
     __builtin_amdgcn_sched_group_barrier(0x100, EACH, 0);
-  }
-}
-
-template <int PRODUCTS, int READS, int VALU>
-__device__ __forceinline__ void weave() {
-#pragma unroll
-  for (int i = 0; i < PRODUCTS; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-    __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
-    if (VALU) __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
   }
 }
 

@@ -378,6 +378,26 @@ def test_attention_strides(device):
             assert torch.equal(got[name], want[name])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [57, 64, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("apart", [1 << 22, (1 << 22) + 8])
+def test_attention_rows_far_apart(dtype, dim, apart):
+    """Rows 2**22 values apart, the widest that is read in place, and more, of
+    a sequence that spans over 2**32 bytes: the same bits as dense rows."""
+    n = 1100 if dtype == torch.bfloat16 else 300
+    base = torch.empty(n * apart, dtype=dtype, device="cuda")
+    far = [base.as_strided((n, 1, dim), (apart, dim, 1), 128 * i).requires_grad_() for i in range(4)]
+    near = attention_inputs((n,), 1, 1, dim, dtype, "cuda")
+    with torch.no_grad():
+        for a, b in zip(far, near):
+            a.copy_(b)
+    cu = ends_of((n,), "cuda")
+    got, want = (attention(*t[:3], t[3].detach(), cu, causal=True) for t in (far, near))
+    for name in want:
+        assert torch.equal(got[name], want[name])
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_attention_gradient_of_a_sum(device):
     """An expanded upstream gradient, and leaves that need none."""
