@@ -6,6 +6,7 @@
 Produces bluefog_amd/_C.*.so (gfx950-only; no CUDA path, no generic
 multi-arch fatbin — this framework targets MI355X)."""
 
+import glob
 import os
 
 from setuptools import setup
@@ -13,6 +14,15 @@ from setuptools import setup
 os.environ.setdefault("PYTORCH_ROCM_ARCH", "gfx950")
 
 from torch.utils.cpp_extension import BuildExtension, CUDAExtension
+
+# Objects of HIP sources carry no record of the headers they include: those
+# older than the newest header are built again.
+_here = os.path.dirname(os.path.abspath(__file__))
+_headers = glob.glob(os.path.join(_here, "bluefog_amd", "csrc", "*.h"))
+_newest = max(map(os.path.getmtime, _headers), default=0)
+for _object in glob.glob(os.path.join(_here, "build", "temp*", "bluefog_amd", "csrc", "*.o")):
+    if os.path.getmtime(_object) < _newest:
+        os.remove(_object)
 
 ext = CUDAExtension(
     name="bluefog_amd._C",
@@ -23,6 +33,7 @@ ext = CUDAExtension(
         "bluefog_amd/csrc/attention.hip",
         "bluefog_amd/csrc/norm.hip",
     ],
+    depends=_headers,
     extra_compile_args={
         "cxx": ["-O3", "-std=c++17"],
         # no packed 32-bit float instructions: some of their forms have given
