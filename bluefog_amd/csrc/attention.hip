@@ -457,6 +457,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kDqWaves<T,
 // over the queries that see them, head by head of the group. S = q k^T and dP
 // lie with a key's queries in the registers of its lane pair, so that P and dS
 // are the operands of dv^T = dO^T P and dk^T = q^T dS as they stand.
+//
+// What dS lost to rounding is multiplied too, as for dq: dk is 1.02 to 1.24 times
+// as far off as its own rounding, 1.41 to 1.51 times without (13195 tokens, 16
+// heads of 128, causal: 0.55 ms, and 0.47 without). P's rounding stays in dv, which
+// is 1.2 to 1.42 times as far off.
 // ---------------------------------------------------------------------------
 
 // A workgroup has 128 keys, four waves of 32, and a step is some queries of
@@ -467,8 +472,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kDqWaves<T,
 //   V_IN_LDS: v's fragments are read again rather than kept in registers
 //   WAVES of a SIMD whose registers it is held to
 //
-// Heads of 128: the sums take 128 registers. Eight waves, two to a SIMD, reach
-// 735 TFLOP/s (16384 tokens, 16 heads, bf16); four with all registers 630.
+// Heads of 128: the sums take 128 registers. Eight waves, two to a SIMD, reached
+// 735 TFLOP/s (16384 tokens, 16 heads, bf16, dS rounded once); four with all registers 630.
 template <typename T, int DP>
 struct DkvShape {
   static constexpr bool kHalf = sizeof(T) == 2, kWide = DP == 128;
@@ -642,14 +647,16 @@ __attribute__((amdgpu_waves_per_eu(DkvShape<T, DP>::kWaves, DkvShape<T, DP>::kWa
         }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const Frag<T> pf = rounded<T>(p + t * 8), df = rounded<T>(ds + t * 8);
+          const Frag<T> pf = rounded<T>(p + t * 8), df = rounded<T>(ds + t * 8), less = rest_of<T>(ds + t * 8, df);
 #pragma unroll
           for (int i = 0; i < kDT; ++i) {
             dv[i] = mma(QG::read_columns(lds[buf][1], columns, sub + t * 16, i), pf, dv[i]);
-            dk[i] = mma(QG::read_columns(lds[buf][0], columns, sub + t * 16, i), df, dk[i]);
+            const Frag<T> qt = QG::read_columns(lds[buf][0], columns, sub + t * 16, i);
+            dk[i] = mma(qt, df, dk[i]);
+            if (sizeof(T) == 2) dk[i] = mma(qt, less, dk[i]);
           }
         }
-        if (sizeof(T) == 2) feed<8, 4 * kDT, 2>();
+        if (sizeof(T) == 2) feed<8, 6 * kDT, 1>();
       }
     }
     loads_done();
