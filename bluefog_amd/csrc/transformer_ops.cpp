@@ -82,8 +82,9 @@ bool any_grad(std::initializer_list<const Tensor*> ts) {
 
 // Whether rows and heads of t are dense along the last dimension, rows are
 // less than 2^22 values apart (a tile's places fit 32 bits) and, where a head
-// fills whole 16-byte accesses, start on one. Other tensors are copied:
-// a copy is cheaper than element-wise reads by every tile.
+// fills whole 16-byte accesses, start on one. Other tensors are copied, dense
+// ones that start elsewhere too: a copy is cheaper than element-wise reads by
+// every tile. Dense rows, of at most 65535 heads of 128, fit as well.
 Tensor readable(const Tensor& t) {
   const int64_t e = t.element_size(), d = t.size(2);
   bool ok = (t.stride(2) == 1 || d == 1) && (t.size(0) == 1 || t.stride(0) <= 1 << 22);
@@ -91,7 +92,7 @@ Tensor readable(const Tensor& t) {
     ok = ok && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
     for (int i = 0; i < 2; ++i) ok = ok && (t.size(i) == 1 || t.stride(i) * e % 16 == 0);
   }
-  return ok ? t : t.contiguous();
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
 BfAttnArgs attn_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu,

@@ -378,6 +378,25 @@ def test_attention_strides(device):
             assert torch.equal(got[name], want[name])
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dim", [40, 64, 57])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_dense_and_misaligned(device, dtype, dim):
+    """Dense tensors, the output's gradient too, that start between 16-byte
+    places: the same bits as aligned ones."""
+    near = attention_inputs((21, 150), 4, 2, dim, dtype, device)
+    cu = ends_of((21, 150), device)
+    moved = []
+    for t in near:
+        flat = torch.empty(t.numel() + 1, dtype=dtype, device=device)
+        flat[1:] = t.detach().flatten()
+        moved.append(flat[1:].view(t.shape).requires_grad_())
+        assert moved[-1].is_contiguous() and moved[-1].data_ptr() % 16
+    got, want = (attention(*t[:3], t[3].detach(), cu, causal=True) for t in (moved, near))
+    for name in want:
+        assert torch.equal(got[name], want[name])
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dim", [57, 64, 128])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
