@@ -344,6 +344,10 @@ inline long units(long tiles, int heads) {
   return (tiles + share - 1) / share * share * heads;
 }
 
+// A launch has fewer tiles. Sequences that overlap can count more, and a sum of
+// the lanes' counts must not leave 32 bits.
+constexpr int kMostTiles = 1 << 24;
+
 struct Work {
   int begin, len;  // rows of the sequence
   int seq, tile;   // tile inside it
@@ -385,7 +389,7 @@ __device__ __forceinline__ Work find_tile(const BfAttnArgs& a, int number, int s
     for (int i = 0; i < chunk; ++i) {  // unguarded, so that the loads go out together
       const int at = lane * chunk + i;
       const int2 b = bounds_of(a, first + min(at, count - 1));
-      sum += at < count ? (b.y - b.x + size - 1) / size : 0;
+      sum = min(sum + (at < count ? (b.y - b.x + size - 1) / size : 0), kMostTiles);
     }
     return sum;
   };

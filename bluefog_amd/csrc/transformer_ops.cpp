@@ -210,11 +210,12 @@ Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
   TORCH_CHECK_VALUE(k.sizes() == v.sizes() && k.size(0) == q.size(0) && k.size(2) == q.size(2),
                     "shapes of q, k and v do not match");
   TORCH_CHECK_VALUE(q.size(2) >= 1 && q.size(2) <= 128, "head dimensions of 1 to 128 are supported, got ", q.size(2));
-  TORCH_CHECK_VALUE(k.size(1) >= 1 && q.size(1) % k.size(1) == 0 && q.size(1) <= 65535,
+  TORCH_CHECK_VALUE(k.size(1) >= 1 && q.size(1) >= 1 && q.size(1) % k.size(1) == 0 && q.size(1) <= 65535,
                     "the number of query heads has to be a multiple of the key/value heads");
   TORCH_CHECK_VALUE(q.size(0) <= 0x7FFF0000ll, "too many tokens");
   TORCH_CHECK_TYPE(cu.scalar_type() == at::kInt, "cu_seqlens has to be int32");
   TORCH_CHECK_VALUE(cu.dim() == 1 && cu.numel() >= 1 && cu.is_contiguous(), "cu_seqlens has to be a dense vector");
+  TORCH_CHECK_VALUE(cu.numel() <= 1 << 24, "too many sequences");
   TORCH_CHECK_VALUE(scale > 0 && std::isfinite(scale), "scale has to be positive and finite, got ", scale);
   check_dropout(q, st, offset, p);
   code_of(q);
@@ -364,8 +365,8 @@ Tensor layer_norm(const Tensor& x, std::optional<Tensor> weight, std::optional<T
                   int64_t seed, int64_t offset) {
   const Tensor r = residual.value_or(Tensor()), st = seed_tensor.value_or(Tensor());
   Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
-  TORCH_CHECK_VALUE(x.is_cuda() && x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= 0x7FFFFFFF,
-                    "layer_norm needs a GPU tensor with a last dimension");
+  TORCH_CHECK_VALUE(x.is_cuda() && x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= 1 << 26,
+                    "layer_norm needs a GPU tensor with a last dimension of 1 to 2^26");
   code_of(x);
   for (const Tensor* t : {&w, &b}) {
     if (!t->defined()) continue;

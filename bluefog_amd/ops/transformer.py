@@ -58,7 +58,7 @@ def packed_attention(
     """Attention inside each sequence of a packed batch.
 
     ``q`` is [tokens, heads, dim], ``k`` and ``v`` are [tokens, kv_heads, dim]
-    with heads a multiple of kv_heads and dim at most 128; rows may be strided
+    with heads (at most 65535) a multiple of kv_heads and dim at most 128; rows may be strided
     (slices of one projection). Sequence b is rows ``cu_seqlens[b]`` to
     ``cu_seqlens[b + 1]``; ``cu_seqlens`` is int32 on the same device, starts
     with 0 and does not decrease (a GPU kernel cannot raise on its values: it
@@ -86,12 +86,14 @@ def packed_attention(
         raise ValueError("shapes of q, k and v do not match")
     if not 1 <= q.shape[2] <= 128:
         raise ValueError(f"head dimensions of 1 to 128 are supported, got {q.shape[2]}")
-    if k.shape[1] < 1 or q.shape[1] % k.shape[1]:
+    if k.shape[1] < 1 or q.shape[1] < 1 or q.shape[1] % k.shape[1] or q.shape[1] > 65535:
         raise ValueError("the number of query heads has to be a multiple of the key/value heads")
     if cu_seqlens.dtype != torch.int32:
         raise TypeError("cu_seqlens has to be int32")
     if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or cu_seqlens.device != q.device:
         raise ValueError("cu_seqlens has to be a dense vector on the same device")
+    if cu_seqlens.numel() > 1 << 24:
+        raise ValueError("too many sequences")
     if not (scale > 0 and math.isfinite(scale)):
         raise ValueError(f"scale has to be positive and finite, got {scale}")
     ends = cu_seqlens.tolist()
@@ -137,7 +139,8 @@ def layer_norm(
     seed: Seed = None,
     offset: int = 0,
 ) -> torch.Tensor:
-    """LayerNorm(residual + dropout(x)) over the last dimension, of any width.
+    """LayerNorm(residual + dropout(x)) over the last dimension, of any width
+    to 2**26.
 
     ``residual`` has x's shape and is of x's type or f32 (a 32-bit residual
     stream under half-precision layers); the result has the residual's type,
@@ -151,8 +154,8 @@ def layer_norm(
             x, weight, bias, eps, residual, dropout_p, seed, value, offset
         )
     _check(x, dropout_p, offset)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError("layer_norm needs a tensor with a last dimension")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= 1 << 26:
+        raise ValueError("layer_norm needs a tensor with a last dimension of 1 to 2^26")
     for t in (weight, bias):
         if t is None:
             continue

@@ -506,6 +506,9 @@ def test_attention_refusals(device):
     refused(ValueError, "do not match", f, q, k, v[:7], cu)
     refused(ValueError, "do not match", f, q, k[..., :8], v[..., :8], cu)
     refused(ValueError, "multiple", f, q[:, :3], k, v, cu)
+    refused(ValueError, "multiple", f, q[:, :0], k, v, cu)
+    refused(ValueError, "multiple", f, q[:, :1].expand(8, 65536, 16), k[:, :1], v[:, :1], cu)
+    refused(ValueError, "too many", f, q, k, v, cu[:1].expand((1 << 24) + 1).contiguous())
     wide = torch.zeros(2, 1, 129, device=device)
     refused(ValueError, "1 to 128", f, wide, wide, wide, ends_of((2,), device))
     refused(TypeError, "int32", f, q, k, v, cu.long())
@@ -526,6 +529,17 @@ def test_attention_refuses_bad_bounds_on_the_cpu():
     q, k, v, _ = attention_inputs((8,), 1, 1, 16, torch.float32, "cpu")
     for ends in ([1, 8], [0, 9], [0, 5, 3], [0, -1]):
         refused(ValueError, "rise", bf.packed_attention, q, k, v, torch.tensor(ends, dtype=torch.int32))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("ends", [[0, 300, 0, 300, 0, 300], [-(1 << 31), (1 << 31) - 1]])
+def test_attention_bad_bounds_are_cut_on_the_gpu(ends, causal):
+    """Bounds that overlap or leave the tensors give what their part inside gives,
+    up to roundings: their number decides over the slices of the sums."""
+    inputs = attention_inputs((300,), 2, 2, 64, torch.bfloat16, "cuda")
+    got = attention(*inputs, torch.tensor(ends, dtype=torch.int32, device="cuda"), causal=causal)
+    close(got, attention_oracle(*inputs, [0, 300], causal, 0.125, 0.0, 0, 0))
 
 
 @pytest.mark.gpu
@@ -682,6 +696,7 @@ def test_norm_refusals(device):
     w, f = torch.ones(16, device=device), bf.layer_norm
     refused(ValueError, "last dimension", f, x[0, 0])
     refused(ValueError, "last dimension", f, x[:, :0])
+    refused(ValueError, "last dimension", f, x[:, :1].expand(4, (1 << 26) + 1))
     refused(ValueError, "vectors", f, x, w[:8])
     refused(ValueError, "vectors", f, x, w, x)
     refused(TypeError, "f32 or of the input's type", f, x, w.half())
