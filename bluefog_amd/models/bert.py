@@ -67,8 +67,9 @@ class BertEmbeddings(nn.Module):
 
         token = torch.arange(input_ids.shape[0], device=input_ids.device, dtype=cu_seqlens.dtype)
         sequence = torch.searchsorted(cu_seqlens, token, right=True) - 1
-        # rows behind the last sequence may lie further than the table goes
-        pos = (token - cu_seqlens[sequence]).clamp_max(self.position.num_embeddings - 1)
+        # rows behind the last sequence may lie further than the table goes, and
+        # bounds on the GPU are not checked
+        pos = (token - cu_seqlens[sequence]).clamp(0, self.position.num_embeddings - 1)
         x = self.word(input_ids) + self.position(pos) + self.token_type(torch.zeros_like(input_ids))
         x = layer_norm(x, self.norm.weight, self.norm.bias, self.norm.eps)
         return counter_dropout(x, p, seed) if p else x

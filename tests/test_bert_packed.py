@@ -147,3 +147,15 @@ def test_bert_packed_refusals():
     refused("rise", ids, ends(0, 20, 10))
     refused("rise", ids, ends(1, 20))
     refused("does not fit", ids, ends(0, 41))
+
+
+@pytest.mark.gpu
+def test_bert_packed_tokens_in_front_of_the_first_sequence():
+    """Bounds on the GPU are not checked: those that start late leave what is in
+    front of them without meaning, and the sequence as it is."""
+    model = _tiny_bert().cuda().eval()
+    ids = torch.randint(0, 97, (60,), generator=torch.Generator().manual_seed(2)).cuda()
+    with torch.no_grad():
+        got = model(ids, cu_seqlens=torch.tensor([13, 50], dtype=torch.int32, device="cuda"))[13:50]
+        alone = model(ids[13:50], cu_seqlens=torch.tensor([0, 37], dtype=torch.int32))
+    assert (got - alone).abs().max() < 1e-5 * alone.abs().max()
