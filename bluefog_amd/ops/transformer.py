@@ -30,6 +30,7 @@ the masks of one seed: give every call of a step its own.
 """
 
 import math
+import operator
 from typing import Optional, Union
 
 import torch
@@ -115,15 +116,15 @@ def packed_attention(
         )
         score = torch.matmul(sq, sk.transpose(1, 2)) * scale
         if causal:
-            i = torch.arange(n)
+            i = torch.arange(n, device=q.device)
             score = score.masked_fill(i > i[:, None], -math.inf)
         prob = torch.softmax(score, 2)
         if dropout_p:
-            prob = _masked(prob, _attention_bits(heads, begin, n, key, offset), dropout_p)
+            prob = _masked(prob, _attention_bits(heads, begin, n, key, offset, q.device), dropout_p)
         parts.append(torch.matmul(prob, sv).transpose(0, 1).to(q.dtype))
     # zeros behind the last sequence, tied to the inputs for the case that no
     # sequence has a row
-    rest = q[ends[-1]:].masked_fill(torch.ones((), dtype=torch.bool), 0.0)
+    rest = q[ends[-1]:].masked_fill(torch.ones((), dtype=torch.bool, device=q.device), 0.0)
     parts.append(rest + k[:0].sum() + v[:0].sum())
     return torch.cat(parts)
 
@@ -176,7 +177,7 @@ def layer_norm(
     wide = x.dtype if x.dtype == torch.float64 else torch.float32
     z = x.to(wide)
     if dropout_p:
-        z = _masked(z, _flat_bits(x.shape, value if seed is None else int(seed), offset), dropout_p)
+        z = _masked(z, _flat_bits(x, value if seed is None else int(seed), offset), dropout_p)
     if residual is not None:
         z = z + residual.to(wide)
     z = z - z.mean(-1, keepdim=True)
@@ -197,7 +198,7 @@ def counter_dropout(x: torch.Tensor, p: float, seed: Seed = None, offset: int = 
         return hip_ext._C.counter_dropout(x, p, seed, value, offset)
     _check(x, p, offset)
     seed, value = _seed(seed, x, p)
-    bits = _flat_bits(x.shape, value if seed is None else int(seed), offset)
+    bits = _flat_bits(x, value if seed is None else int(seed), offset)
     wide = x.dtype if x.dtype == torch.float64 else torch.float32
     return _masked(x.to(wide), bits, p).to(x.dtype)
 
@@ -217,9 +218,13 @@ def _seed(seed: Seed, like: torch.Tensor, p: float):
         if seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != like.device:
             raise ValueError("seed has to be an int or one int64 on the input's device")
         return seed, 0
+    try:
+        seed = operator.index(seed)
+    except TypeError:
+        raise ValueError("seed has to be an int or one int64 on the input's device") from None
     if not -(1 << 63) <= seed < 1 << 63:
         raise ValueError(f"seed has to fit 64 bits, got {seed}")
-    return None, int(seed)
+    return None, seed
 
 
 def _check(x: torch.Tensor, p: float, offset: int) -> None:
@@ -248,19 +253,19 @@ def _philox(c0, c1, c2, c3, key: int) -> torch.Tensor:
     return torch.stack((words & 0xFFFF, words >> 16), -1).flatten(-2)
 
 
-def _flat_bits(shape, key: int, offset: int) -> torch.Tensor:
-    n = math.prod(shape)
-    block = torch.arange((n + 7) // 8)
+def _flat_bits(x: torch.Tensor, key: int, offset: int) -> torch.Tensor:
+    n = x.numel()
+    block = torch.arange((n + 7) // 8, device=x.device)
     zero = torch.zeros_like(block)
     bits = _philox(block & _M32, block >> 32, zero, zero + offset, key)
-    return bits.flatten()[:n].view(shape)
+    return bits.flatten()[:n].view(x.shape)
 
 
-def _attention_bits(heads: int, begin: int, n: int, key: int, offset: int) -> torch.Tensor:
+def _attention_bits(heads: int, begin: int, n: int, key: int, offset: int, device) -> torch.Tensor:
     """[heads, n, n] for the sequence that starts in row ``begin``."""
-    call = torch.arange(2 * ((n + 15) // 16))
-    row = begin + torch.arange(n)[:, None]
-    head = torch.arange(heads)[:, None, None]
+    call = torch.arange(2 * ((n + 15) // 16), device=device)
+    row = begin + torch.arange(n, device=device)[:, None]
+    head = torch.arange(heads, device=device)[:, None, None]
     bits = _philox(call, row, head, torch.full_like(call, offset), key)
     # [.., 16 keys, quad parity, (key // 8 % 2, key % 4)] -> keys in order
     bits = bits.unflatten(3, (2, 4)).unflatten(2, (-1, 2)).transpose(3, 4)

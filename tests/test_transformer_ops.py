@@ -15,6 +15,7 @@ import pytest
 import torch
 
 import bluefog_amd as bf
+from bluefog_amd.ops import hip_ext
 
 F32 = 2.0 ** -24
 LEAST = 2.0 ** -126
@@ -520,6 +521,7 @@ def test_attention_refusals(device):
     refused(ValueError, "offset", f, q, k, v, cu, dropout_p=0.1, seed=1, offset=1 << 32)
     refused(ValueError, "offset", f, q, k, v, cu, dropout_p=0.1, seed=1, offset=-1)
     refused(ValueError, "seed", f, q, k, v, cu, dropout_p=0.1, seed=torch.zeros(2, dtype=torch.int64, device=device))
+    refused(ValueError, "seed", f, q, k, v, cu, dropout_p=0.1, seed=1.5)
     refused(ValueError, "64 bits", f, q, k, v, cu, dropout_p=0.1, seed=1 << 63)
     whole = torch.zeros(8, 1, 16, dtype=torch.int32, device=device)
     refused(TypeError, "f16", f, whole, whole, whole, cu)
@@ -878,3 +880,31 @@ def test_in_captured_graphs():
         for got, w in zip(outs, want):
             for a, b in zip(got, w):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_torch_code_on_the_gpu(monkeypatch):
+    """Without the extension: an error, or the torch code when that is asked for,
+    with the same masks."""
+    q, k, v, dout = attention_inputs((9, 40), 4, 2, 16, torch.float32, "cuda", spare=3)
+    cu, x = ends_of((9, 40), "cuda"), torch.randn(5, 24, device="cuda", requires_grad=True)
+    kw = dict(dropout_p=0.3, seed=5, offset=2)
+
+    def results():
+        y = bf.counter_dropout(x, 0.3, 5, 2)
+        got = attention(q, k, v, dout, cu, causal=True, **kw)
+        return {**got, "y": y, "norm": bf.layer_norm(x, residual=x, **kw)}
+
+    native = results()
+    monkeypatch.setattr(hip_ext, "_C", None)
+    with pytest.raises(RuntimeError, match="requires the native HIP"):
+        results()
+    monkeypatch.setenv("BLUEFOG_ALLOW_TORCH_FALLBACK", "1")
+    want = attention_oracle(q, k, v, dout, cu.tolist(), True, 0.25, 0.3, 5, 2)
+    plain = results()
+    close({n: plain[n] for n in want}, want)
+    close({n: native[n] for n in want}, want)
+    assert torch.equal(native["y"], plain["y"])
+    # both in 32 bits: sums of 24 values below 16 move the mean by 24 F32 * 16 at most and 1 / sigma (above 0.5
+    # of values of size 1) by 26 F32 of itself, of results below 5
+    torch.testing.assert_close(native["norm"], plain["norm"], rtol=0, atol=2 * (2 * 24 * 16 + 5 * 26) * F32)
