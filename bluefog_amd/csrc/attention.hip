@@ -506,7 +506,7 @@ __attribute__((amdgpu_waves_per_eu(DkvShape<T, DP>::kWaves, DkvShape<T, DP>::kWa
   constexpr int BM = 32 * SPLIT * SUBS;  // queries of a step
   constexpr int kSteps = DP / 16, kDT = DP / 32;
   constexpr bool V_IN_LDS = Shape::kVInLds;
-  constexpr bool kHide = sizeof(T) == 2 && DP == 128;  // 670 TFLOP/s without, 710 with
+  constexpr bool kHide = sizeof(T) == 2 && DP == 128;  // 670 TFLOP/s without, 710 with (dS rounded once)
   typedef Tile<T, BM, DP, THREADS, VEC> QG;
   typedef Tile<T, kK, DP, THREADS, VEC> Values;
   __shared__ __align__(1024) char lds[2][2][QG::kBytes];
@@ -771,9 +771,9 @@ extern "C" {
 // and dv) over all queries of its keys and head group. Few tokens or few key
 // heads leave few workgroups, which then take a share of that axis each; a second
 // kernel joins the shares, from 32-bit sums in memory. That pays up to about two
-// workgroups of a CU: forward and backward of 1689 tokens (10/2 heads of 80)
-// take 137 us with slices and 417 without, but those of 4 K tokens under 8
-// heads of 128 take 469 us with a target of 512 workgroups, 576 with 1024.
+// workgroups of a CU. With dS rounded once, forward and backward of 1689 tokens
+// (10/2 heads of 80) took 137 us with slices and 417 without, but those of 4 K
+// tokens under 8 heads of 128 took 469 us with a target of 512 workgroups, 576 with 1024.
 constexpr long kWanted = 512;
 
 int bf_attn_key_slices(const BfAttnArgs* a, int dtype) {

@@ -64,15 +64,6 @@ __device__ __forceinline__ Acc mma(Frag<float> a, Frag<float> b, Acc c) {
   return c;
 }
 
-// whether a fragment holds an infinity or what is no number
-template <typename F>
-__device__ __forceinline__ int not_finite(F f) {
-  int found = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) found |= !(fabsf(static_cast<float>(f[i])) < INFINITY);
-  return found;
-}
-
 // inner position of accumulator register r
 __device__ __forceinline__ int row_of(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
 
