@@ -2,13 +2,17 @@
 //
 // Torch side of the transformer training operators: argument checks, strides,
 // workspaces, and the autograd nodes. The nodes are C++ so that a small call
-// costs microseconds and the backward pass runs without the interpreter.
+// costs microseconds and the backward pass runs without the interpreter. The
+// operators are known to torch's dispatcher, so that a trace records a call of
+// theirs and not the allocation that it returns.
 
 #include <torch/extension.h>
 
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/library.h>
 
 #include <optional>
 
@@ -199,7 +203,7 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
 };
 
 Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu,
-                        double scale, bool causal, double p, std::optional<Tensor> seed_tensor,
+                        double scale, bool causal, double p, const std::optional<Tensor>& seed_tensor,
                         int64_t seed, int64_t offset) {
   const Tensor st = seed_tensor.value_or(Tensor());
   TORCH_CHECK_VALUE(q.dim() == 3 && k.dim() == 3 && v.dim() == 3, "q, k and v have to be [tokens, heads, dim]");
@@ -220,7 +224,6 @@ Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
   check_dropout(q, st, offset, p);
   code_of(q);
   const bool grad = any_grad({&q, &k, &v});
-  py::gil_scoped_release nogil;
   const Tensor rq = readable(q), rk = readable(k), rv = readable(v);
   if (grad) return PackedAttention::apply(rq, rk, rv, cu, seed_tensor, scale, causal, p, seed, offset);
   return attn_forward(rq, rk, rv, cu, scale, causal, dropout_args(st, seed, offset, p), nullptr, nullptr);
@@ -360,8 +363,8 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   }
 };
 
-Tensor layer_norm(const Tensor& x, std::optional<Tensor> weight, std::optional<Tensor> bias, double eps,
-                  std::optional<Tensor> residual, double p, std::optional<Tensor> seed_tensor,
+Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, double eps,
+                  const std::optional<Tensor>& residual, double p, const std::optional<Tensor>& seed_tensor,
                   int64_t seed, int64_t offset) {
   const Tensor r = residual.value_or(Tensor()), st = seed_tensor.value_or(Tensor());
   Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
@@ -385,7 +388,6 @@ Tensor layer_norm(const Tensor& x, std::optional<Tensor> weight, std::optional<T
   TORCH_CHECK_VALUE(eps >= 0 && std::isfinite(eps), "eps has to be finite and not negative, got ", eps);
   check_dropout(x, st, offset, p);
   const bool grad = any_grad({&x, &r, &w, &b});
-  py::gil_scoped_release nogil;
   if (w.defined()) w = w.contiguous();
   if (b.defined()) b = b.contiguous();
   if (grad) {
@@ -430,21 +432,41 @@ struct CounterDropout : torch::autograd::Function<CounterDropout> {
   }
 };
 
-Tensor counter_dropout(const Tensor& x, double p, std::optional<Tensor> seed_tensor, int64_t seed, int64_t offset) {
+Tensor counter_dropout(const Tensor& x, double p, const std::optional<Tensor>& seed_tensor, int64_t seed,
+                       int64_t offset) {
   const Tensor st = seed_tensor.value_or(Tensor());
   TORCH_CHECK_VALUE(x.is_cuda(), "counter_dropout needs a GPU tensor");
   check_dropout(x, st, offset, p);
   code_of(x);
   const bool grad = any_grad({&x});
-  py::gil_scoped_release nogil;
   if (grad) return CounterDropout::apply(x, seed_tensor, p, seed, offset);
   return masked(x, dropout_args(st, seed, offset, p));
 }
 
+// the operator `name` as torch's dispatcher calls it, with F's arguments
+template <auto F>
+struct Dispatched;
+template <typename... Args, Tensor (*F)(Args...)>
+struct Dispatched<F> {
+  static void bind(py::module& m, const char* name, const char* doc) {
+    const auto op =
+        c10::Dispatcher::singleton().findSchemaOrThrow((std::string("bluefog_amd::") + name).c_str(), "").typed<Tensor(Args...)>();
+    m.def(name, [op](Args... args) { return op.call(args...); }, py::call_guard<py::gil_scoped_release>(), doc);
+  }
+};
+
 }  // namespace
 
+TORCH_LIBRARY(bluefog_amd, m) {
+  m.def("packed_attention(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens, float scale, bool causal, float dropout_p, "
+        "Tensor? seed_tensor, int seed, int offset) -> Tensor", &packed_attention);
+  m.def("layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps, Tensor? residual, float dropout_p, "
+        "Tensor? seed_tensor, int seed, int offset) -> Tensor", &layer_norm);
+  m.def("counter_dropout(Tensor x, float p, Tensor? seed_tensor, int seed, int offset) -> Tensor", &counter_dropout);
+}
+
 void bf_register_transformer_ops(py::module& m) {
-  m.def("packed_attention", &packed_attention, "softmax(scale q k^T) v inside packed sequences");
-  m.def("layer_norm", &layer_norm, "LayerNorm(residual + dropout(x))");
-  m.def("counter_dropout", &counter_dropout, "x * keep / (1 - p), the mask from a counter");
+  Dispatched<&packed_attention>::bind(m, "packed_attention", "softmax(scale q k^T) v inside packed sequences");
+  Dispatched<&layer_norm>::bind(m, "layer_norm", "LayerNorm(residual + dropout(x))");
+  Dispatched<&counter_dropout>::bind(m, "counter_dropout", "x * keep / (1 - p), the mask from a counter");
 }

@@ -908,3 +908,62 @@ def test_torch_code_on_the_gpu(monkeypatch):
     # both in 32 bits: sums of 24 values below 16 move the mean by 24 F32 * 16 at most and 1 / sigma (above 0.5
     # of values of size 1) by 26 F32 of itself, of results below 5
     torch.testing.assert_close(native["norm"], plain["norm"], rtol=0, atol=2 * (2 * 24 * 16 + 5 * 26) * F32)
+
+
+# ---------------------------------------------------------------------------
+# torch's other ways to call a function
+# ---------------------------------------------------------------------------
+
+
+def calls_of_all(device, dtype=torch.float32):
+    """[(function of tensors, those tensors)], every differentiable argument among them."""
+    q, k, v, _ = (t.detach() for t in attention_inputs((5, 9), 4, 2, 16, dtype, device))
+    x, r, w, b, _ = (t.detach() for t in norm_inputs((6, 24), dtype, device, residual=dtype, weights=dtype))
+    cu, kw = ends_of((5, 9), device), dict(dropout_p=0.3, seed=5, offset=2)
+    return [
+        (lambda q, k, v: bf.packed_attention(q, k, v, cu, causal=True, **kw), (q, k, v)),
+        (lambda x, r, w, b: bf.layer_norm(x, w, b, residual=r, **kw), (x, r, w, b)),
+        (lambda x: bf.counter_dropout(x, 0.3, 5, 2), (x,)),
+    ]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("which", range(3))
+def test_traced(device, which):
+    """A trace holds the operator, not the memory of its first result: new inputs
+    give what the function gives, gradients too."""
+    f, args = calls_of_all(device)[which]
+    traced = torch.jit.trace(f, args)
+    if device == "cuda":
+        assert "bluefog_amd::" in str(traced.graph)
+    for factor in (1.0, -2.0, 0.5):
+        new = [(t * factor).requires_grad_() for t in args]
+        got, want = traced(*new), f(*new)
+        assert torch.equal(got, want)
+        for a, b in zip(torch.autograd.grad(got.sum(), new), torch.autograd.grad(want.sum(), new)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_traced_seed(device):
+    """A seed that is a tensor is an input of the trace."""
+    x, seed = torch.ones(1000, device=device), torch.tensor([3], device=device)
+    if device == "cpu":
+        pytest.skip("the torch code reads the seed on the host: a trace keeps its value")
+    traced = torch.jit.trace(lambda x, s: bf.counter_dropout(x, 0.5, s), (x, seed))
+    for s in (3, 4):
+        assert torch.equal(traced(x, seed.fill_(s)), bf.counter_dropout(x, 0.5, s))
+
+
+@pytest.mark.gpu
+def test_mapped_over_a_dimension():
+    """torch.vmap runs the operator slice by slice, and differentiates through it."""
+    x = torch.randn(3, 4, 32, device="cuda")
+    w = torch.rand(32, device="cuda", requires_grad=True)
+    assert torch.equal(torch.vmap(lambda t: bf.counter_dropout(t, 0.3, 5))(x),
+                       torch.stack([bf.counter_dropout(t, 0.3, 5) for t in x]))
+    got, want = torch.vmap(lambda t: bf.layer_norm(t, w))(x), bf.layer_norm(x, w)
+    assert torch.equal(got, want)
+    a, b = (torch.autograd.grad(y.sum(), w)[0] for y in (got, want))
+    # sums of 12 terms of size below 8 in another order
+    assert (a - b).abs().max() <= 2 * 12 * 12 * 8 * F32
