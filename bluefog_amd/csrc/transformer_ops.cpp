@@ -46,6 +46,14 @@ void check(hipError_t e, const char* what) {
   TORCH_CHECK(e == hipSuccess, "bluefog_amd ", what, ": ", hipGetErrorString(e));
 }
 
+// A fake tensor, or one whose storage was freed, is a GPU tensor with nowhere to
+// read: a kernel would fault.
+void with_memory(const char* what, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->numel() || t->const_data_ptr(), "bluefog_amd ", what,
+                                " needs tensors with memory: no fake ones, none whose storage was freed");
+}
+
 // The kernels' results have no graph of their own: a second derivative
 // through them would silently be zero.
 void once_only(const char* what) {
@@ -136,6 +144,7 @@ Tensor attn_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Ten
   if (lse) *lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
   if (rest && q.scalar_type() != at::kFloat) *rest = at::empty(out.sizes(), q.options());
   if (out.numel() == 0) return out;
+  with_memory("packed_attention", {&out});  // a mode may make new tensors fake
   BfAttnArgs a = attn_args(q, k, v, cu, scale, causal, drop);
   a.o = out.data_ptr();
   a.lse = lse ? lse->data_ptr<float>() : nullptr;
@@ -169,6 +178,7 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
     if (!grads[0].defined()) return none;
     const variable_list s = ctx->get_saved_variables();
     const Tensor &q = s[0], &k = s[1], &v = s[2], &cu = s[3], &seed_tensor = s[4], &out = s[5], &lse = s[6], &rest = s[7];
+    with_memory("packed_attention backward", {&q, &k, &v, &cu, &seed_tensor, &out, &lse, &rest, &grads[0]});
     c10::DeviceGuard guard(q.device());
     const bool need_dq = ctx->needs_input_grad(0);
     const bool need_dkv = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
@@ -176,6 +186,7 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
     Tensor dq = at::empty(out.sizes(), out.options());
     Tensor dk = at::empty(k.sizes(), k.options(), at::MemoryFormat::Contiguous);
     Tensor dv = at::empty(v.sizes(), v.options(), at::MemoryFormat::Contiguous);
+    with_memory("packed_attention backward", {&dq});
     if (out.numel()) {
       Tensor delta = at::empty(lse.sizes(), lse.options());
       BfAttnArgs a = attn_args(q, k, v, cu, ctx->saved_data["scale"].toDouble(),
@@ -223,6 +234,7 @@ Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
   TORCH_CHECK_VALUE(scale > 0 && std::isfinite(scale), "scale has to be positive and finite, got ", scale);
   check_dropout(q, st, offset, p);
   code_of(q);
+  with_memory("packed_attention", {&q, &k, &v, &cu, &st});
   const bool grad = any_grad({&q, &k, &v});
   const Tensor rq = readable(q), rk = readable(k), rv = readable(v);
   if (grad) return PackedAttention::apply(rq, rk, rv, cu, seed_tensor, scale, causal, p, seed, offset);
@@ -277,6 +289,7 @@ Tensor norm_forward(const Tensor& x, const Tensor& r, const Tensor& weight, cons
     a.rstd = rstd->data_ptr<float>();
   }
   if (a.rows == 0) return y;
+  with_memory("layer_norm", {&y});  // a mode may make new tensors fake
   const auto [rx, x_row] = as_rows(x);
   a.x = rx.const_data_ptr(), a.x_row = x_row;
   Tensor hold;
@@ -315,6 +328,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     if (!grads[0].defined()) return got;
     const variable_list s = ctx->get_saved_variables();
     const Tensor &x = s[0], &r = s[1], &weight = s[2], &bias = s[3], &seed_tensor = s[4];
+    with_memory("layer_norm backward", {&x, &r, &weight, &bias, &seed_tensor, &s[5], &s[6], &grads[0]});
     c10::DeviceGuard guard(x.device());
     BfNormArgs a = norm_args(x, r, weight, bias, ctx->saved_data["eps"].toDouble(),
                              dropout_args(seed_tensor, ctx->saved_data["seed"].toInt(),
@@ -331,6 +345,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     }
     if (weight.defined() && ctx->needs_input_grad(w_edge)) got[2] = at::empty_like(weight);
     if (bias.defined() && ctx->needs_input_grad(b_edge)) got[3] = at::empty_like(bias);
+    with_memory("layer_norm backward", {&got[0], &got[1], &got[2], &got[3]});
     if (a.rows == 0) {
       for (int i = 2; i < 4; ++i)
         if (got[i].defined()) got[i].zero_();
@@ -387,6 +402,7 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const st
   }
   TORCH_CHECK_VALUE(eps >= 0 && std::isfinite(eps), "eps has to be finite and not negative, got ", eps);
   check_dropout(x, st, offset, p);
+  with_memory("layer_norm", {&x, &r, &w, &b, &st});
   const bool grad = any_grad({&x, &r, &w, &b});
   if (w.defined()) w = w.contiguous();
   if (b.defined()) b = b.contiguous();
@@ -405,6 +421,7 @@ Tensor masked(const Tensor& x, const BfDropout& d) {
   c10::DeviceGuard guard(x.device());
   const Tensor in = x.contiguous();
   Tensor y = at::empty(in.sizes(), in.options(), at::MemoryFormat::Contiguous);
+  with_memory("counter_dropout", {&in, &y});
   if (in.numel())
     check(bf_dropout(y.data_ptr(), in.const_data_ptr(), in.numel(), code_of(in), &d, stream_of(in)),
           "counter_dropout");
@@ -426,7 +443,9 @@ struct CounterDropout : torch::autograd::Function<CounterDropout> {
     once_only("counter_dropout");
     variable_list got(5);
     if (!grads[0].defined()) return got;
-    got[0] = masked(grads[0], dropout_args(ctx->get_saved_variables()[0], ctx->saved_data["seed"].toInt(),
+    const Tensor seed_tensor = ctx->get_saved_variables()[0];
+    with_memory("counter_dropout backward", {&seed_tensor});
+    got[0] = masked(grads[0], dropout_args(seed_tensor, ctx->saved_data["seed"].toInt(),
                                            ctx->saved_data["offset"].toInt(), ctx->saved_data["p"].toDouble()));
     return got;
   }
@@ -438,6 +457,7 @@ Tensor counter_dropout(const Tensor& x, double p, const std::optional<Tensor>& s
   TORCH_CHECK_VALUE(x.is_cuda(), "counter_dropout needs a GPU tensor");
   check_dropout(x, st, offset, p);
   code_of(x);
+  with_memory("counter_dropout", {&x, &st});
   const bool grad = any_grad({&x});
   if (grad) return CounterDropout::apply(x, seed_tensor, p, seed, offset);
   return masked(x, dropout_args(st, seed, offset, p));

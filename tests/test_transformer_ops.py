@@ -955,6 +955,47 @@ def test_traced_seed(device):
         assert torch.equal(traced(x, seed.fill_(s)), bf.counter_dropout(x, 0.5, s))
 
 
+def test_fake_tensors_are_refused():
+    """They say that they are on a GPU and have no memory: a kernel would read
+    address 0. Nothing is launched, so this runs without a GPU as well."""
+    from torch._subclasses import FakeTensorMode
+
+    if not hip_ext.has_extension():
+        pytest.skip("the native extension is not built")
+    with FakeTensorMode():
+        q, x = torch.empty(8, 2, 16, device="cuda"), torch.empty(4, 24, device="cuda")
+        cu, seed = torch.empty(2, dtype=torch.int32, device="cuda"), torch.empty(1, dtype=torch.int64, device="cuda")
+        for needs in (False, True):
+            q.requires_grad_(needs)
+            x.requires_grad_(needs)
+            refused(NotImplementedError, "memory", bf.packed_attention, q, q, q, cu)
+            refused(NotImplementedError, "memory", bf.packed_attention, q, q, q, cu, dropout_p=0.1, seed=seed)
+            refused(NotImplementedError, "memory", bf.layer_norm, x, residual=x)
+            refused(NotImplementedError, "memory", bf.counter_dropout, x, 0.1, seed)
+
+
+@pytest.mark.gpu
+def test_tensors_without_memory_are_refused():
+    """Inputs and gradients whose storage was freed, and results that a mode
+    makes fake, in both directions."""
+    from torch._subclasses import FakeTensorMode
+
+    def freed(t):
+        t = t.clone()
+        t.untyped_storage().resize_(0)
+        assert t.data_ptr() == 0
+        return t
+
+    for f, args in calls_of_all("cuda"):
+        for i, t in enumerate(args):
+            refused(NotImplementedError, "memory", f, *args[:i], freed(t), *args[i + 1:])
+        with FakeTensorMode(allow_non_fake_inputs=True):
+            refused(NotImplementedError, "memory", f, *args)
+        leaf = args[0].clone().requires_grad_()
+        out = f(leaf, *args[1:])
+        refused(NotImplementedError, "memory", torch.autograd.grad, out, leaf, freed(torch.ones_like(out)))
+
+
 @pytest.mark.gpu
 def test_mapped_over_a_dimension():
     """torch.vmap runs the operator slice by slice, and differentiates through it."""
