@@ -54,11 +54,19 @@ void with_memory(const char* what, std::initializer_list<const Tensor*> ts) {
                                 " needs tensors with memory: no fake ones, none whose storage was freed");
 }
 
+// The kernels take no tangents along: the derivative would silently be lost.
+void no_tangents(const char* what, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), "bluefog_amd ", what,
+                                " has no forward-mode derivative");
+}
+
 // The kernels' results have no graph of their own: a second derivative
 // through them would silently be zero.
-void once_only(const char* what) {
+void once_only(const char* what, const Tensor& grad) {
   TORCH_CHECK(!at::GradMode::is_enabled(), "bluefog_amd ", what,
               " is differentiable once: create_graph=True is not supported");
+  no_tangents(what, {&grad});
 }
 
 BfDropout dropout_args(const Tensor& seed_tensor, int64_t seed, int64_t offset,
@@ -173,7 +181,7 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    once_only("packed_attention");
+    once_only("packed_attention", grads[0]);
     variable_list none(10);
     if (!grads[0].defined()) return none;
     const variable_list s = ctx->get_saved_variables();
@@ -235,6 +243,7 @@ Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
   check_dropout(q, st, offset, p);
   code_of(q);
   with_memory("packed_attention", {&q, &k, &v, &cu, &st});
+  no_tangents("packed_attention", {&q, &k, &v});
   const bool grad = any_grad({&q, &k, &v});
   const Tensor rq = readable(q), rk = readable(k), rv = readable(v);
   if (grad) return PackedAttention::apply(rq, rk, rv, cu, seed_tensor, scale, causal, p, seed, offset);
@@ -323,7 +332,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    once_only("layer_norm");
+    once_only("layer_norm", grads[0]);
     variable_list got(9);
     if (!grads[0].defined()) return got;
     const variable_list s = ctx->get_saved_variables();
@@ -403,6 +412,7 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const st
   TORCH_CHECK_VALUE(eps >= 0 && std::isfinite(eps), "eps has to be finite and not negative, got ", eps);
   check_dropout(x, st, offset, p);
   with_memory("layer_norm", {&x, &r, &w, &b, &st});
+  no_tangents("layer_norm", {&x, &r, &w, &b});
   const bool grad = any_grad({&x, &r, &w, &b});
   if (w.defined()) w = w.contiguous();
   if (b.defined()) b = b.contiguous();
@@ -440,7 +450,7 @@ struct CounterDropout : torch::autograd::Function<CounterDropout> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    once_only("counter_dropout");
+    once_only("counter_dropout", grads[0]);
     variable_list got(5);
     if (!grads[0].defined()) return got;
     const Tensor seed_tensor = ctx->get_saved_variables()[0];
@@ -458,6 +468,7 @@ Tensor counter_dropout(const Tensor& x, double p, const std::optional<Tensor>& s
   check_dropout(x, st, offset, p);
   code_of(x);
   with_memory("counter_dropout", {&x, &st});
+  no_tangents("counter_dropout", {&x});
   const bool grad = any_grad({&x});
   if (grad) return CounterDropout::apply(x, seed_tensor, p, seed, offset);
   return masked(x, dropout_args(st, seed, offset, p));

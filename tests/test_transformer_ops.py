@@ -927,6 +927,42 @@ def calls_of_all(device, dtype=torch.float32):
     ]
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", range(3))
+def test_forward_mode_is_refused_on_the_gpu(which):
+    """The kernels take no tangents along: an argument that carries one is refused,
+    whether or not it requires a gradient, in the backward pass too."""
+    from torch.autograd import forward_ad
+
+    f, args = calls_of_all("cuda")[which]
+    leaf = args[0].clone().requires_grad_()
+    with forward_ad.dual_level():
+        for i, t in enumerate(args):
+            for needs in (False, True):
+                dual = forward_ad.make_dual(t.clone().requires_grad_(needs), torch.ones_like(t))
+                refused(NotImplementedError, "forward-mode", f, *args[:i], dual, *args[i + 1:])
+                with torch.no_grad():
+                    refused(NotImplementedError, "forward-mode", f, *args[:i], dual, *args[i + 1:])
+        out = f(leaf, *args[1:])
+        dual = forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
+        refused(NotImplementedError, "forward-mode", torch.autograd.grad, out, leaf, dual)
+
+
+@pytest.mark.parametrize("which", range(3))
+def test_forward_mode_on_the_cpu(which):
+    """The torch code's tangents against J t from two backward passes, in 64 bits:
+    sums of at most 40 terms of size below 100."""
+    from torch.autograd import forward_ad
+
+    f, args = calls_of_all("cpu", torch.float64)[which]
+    g = torch.Generator().manual_seed(8)
+    along = tuple(torch.randn(t.shape, generator=g, dtype=t.dtype) for t in args)
+    with forward_ad.dual_level():
+        got = forward_ad.unpack_dual(f(*(forward_ad.make_dual(t, e) for t, e in zip(args, along)))).tangent
+    _, want = torch.autograd.functional.jvp(f, args, along)
+    torch.testing.assert_close(got, want, rtol=0, atol=40 * 100 * 2.0 ** -52)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("which", range(3))
 def test_traced(device, which):
