@@ -26,6 +26,8 @@ using namespace bf_attn;
 // last ones are used.
 // ---------------------------------------------------------------------------
 
+constexpr int kRows = 128;  // queries, or keys of dk and dv, of a workgroup
+
 template <typename T>
 constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;  // keys of a tile
 
@@ -53,7 +55,7 @@ constexpr float kSlack = 8.f;
 
 template <typename T, int DP, bool VEC, bool DROP>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kFwdWaves<T, DP>, kFwdWaves<T, DP>))) void attn_fwd_k(BfAttnArgs a) {
-  constexpr int kQ = 128, BN = kKeys<T>, kSub = BN / 32, kSteps = DP / 16, kDT = DP / 32;
+  constexpr int kQ = kRows, BN = kKeys<T>, kSub = BN / 32, kSteps = DP / 16, kDT = DP / 32;
   typedef Tile<T, BN, DP, 256, VEC> KV;
   __shared__ __align__(1024) char lds[2][2][KV::kBytes];
   const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
@@ -319,7 +321,7 @@ __device__ __forceinline__ void rescale(Acc (&acc)[TILES], float& factor, const 
 
 template <typename T, int DP, bool VEC, bool DROP>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kDqWaves<T, DP>, kDqWaves<T, DP>))) void attn_dq_k(BfAttnArgs a) {
-  constexpr int kQ = 128, BN = kKeys<T>, kSub = BN / 32, kSteps = DP / 16, kDT = DP / 32;
+  constexpr int kQ = kRows, BN = kKeys<T>, kSub = BN / 32, kSteps = DP / 16, kDT = DP / 32;
   typedef Tile<T, BN, DP, 256, VEC> KV;
   __shared__ __align__(1024) char lds[2][2][KV::kBytes];
   const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
@@ -502,7 +504,7 @@ template <typename T, int DP, bool VEC, bool DROP>
 __global__ __launch_bounds__((256 * DkvShape<T, DP>::kSplit))
 __attribute__((amdgpu_waves_per_eu(DkvShape<T, DP>::kWaves, DkvShape<T, DP>::kWaves))) void attn_dkv_k(BfAttnArgs a) {
   typedef DkvShape<T, DP> Shape;
-  constexpr int kK = 128, SPLIT = Shape::kSplit, SUBS = Shape::kSubs, THREADS = 256 * SPLIT;
+  constexpr int kK = kRows, SPLIT = Shape::kSplit, SUBS = Shape::kSubs, THREADS = 256 * SPLIT;
   constexpr int BM = 32 * SPLIT * SUBS;  // queries of a step
   constexpr int kSteps = DP / 16, kDT = DP / 32;
   constexpr bool V_IN_LDS = Shape::kVInLds;
@@ -699,12 +701,13 @@ __global__ __launch_bounds__(256) void attn_fold_k(T* first, T* second, const fl
     if (u < n) out[u] = static_cast<T>(sum[u]);
 }
 
-constexpr long kMostGroups = 0xFFFFFF;  // of 256 threads: a launch has less than 2^32
+__global__ __launch_bounds__(1024) void attn_table_k(BfAttnArgs a, int* table) { make_table(a, table, kRows); }
+
+constexpr long kMostThreads = 0xFFFFFFFF;  // of a launch
 
 template <typename T>
 hipError_t fold(void* first, void* second, const float* partial, long all, int slices, hipStream_t stream) {
-  const long blocks = (all + 1023) / 1024;
-  if (blocks > kMostGroups) return hipErrorInvalidValue;
+  const long blocks = (all + 1023) / 1024;  // slices have few rows: far from kMostThreads
   hipLaunchKernelGGL(attn_fold_k<T>, dim3(blocks, second ? 2 : 1), dim3(256), 0, stream, static_cast<T*>(first),
                      static_cast<T*>(second), partial, all, slices);
   return hipGetLastError();
@@ -712,14 +715,13 @@ hipError_t fold(void* first, void* second, const float* partial, long all, int s
 
 template <typename T, int DP, bool VEC>
 hipError_t fwd(const BfAttnArgs& a, hipStream_t stream) {
-  const long groups = units(most_tiles(a, 128) * a.key_slices, a.heads);
-  if (groups > kMostGroups) return hipErrorInvalidValue;
+  const long groups = units(most_tiles(a, kRows) * a.key_slices, a.heads);
+  if (groups * 256 > kMostThreads) return hipErrorInvalidValue;
   if (a.drop.threshold) hipLaunchKernelGGL((attn_fwd_k<T, DP, VEC, true>), dim3(groups), dim3(256), 0, stream, a);
   else hipLaunchKernelGGL((attn_fwd_k<T, DP, VEC, false>), dim3(groups), dim3(256), 0, stream, a);
   if (hipError_t e = hipGetLastError()) return e;
   if (a.key_slices == 1) return hipSuccess;
   const long blocks = (static_cast<long>(a.rows) * a.heads * ((a.dim + 3) / 4) + 255) / 256;
-  if (blocks > kMostGroups) return hipErrorInvalidValue;
   hipLaunchKernelGGL(attn_join_k<T>, dim3(blocks), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
@@ -732,16 +734,17 @@ hipError_t fwd(const BfAttnArgs& a, hipStream_t stream) {
 
 template <typename T, int DP, bool VEC, bool DROP>
 hipError_t bwd(const BfAttnArgs& a, bool need_dkv, hipStream_t stream) {
-  const long groups = units(most_tiles(a, 128) * a.key_slices, a.heads);
-  const long shared = units(most_tiles(a, 128) * a.query_slices, a.kv_heads);
-  if (groups > kMostGroups || shared > kMostGroups / 2) return hipErrorInvalidValue;
+  constexpr int kThreads = 256 * DkvShape<T, DP>::kSplit;
+  const long groups = units(most_tiles(a, kRows) * a.key_slices, a.heads);
+  const long shared = units(most_tiles(a, kRows) * a.query_slices, a.kv_heads);
+  if (groups * 256 > kMostThreads || shared * kThreads > kMostThreads) return hipErrorInvalidValue;
   hipLaunchKernelGGL((attn_dq_k<T, DP, VEC, DROP>), dim3(groups), dim3(256), 0, stream, a);
   if (hipError_t e = hipGetLastError()) return e;
   if (a.key_slices > 1)
     if (hipError_t e = fold<T>(a.dq, nullptr, a.partial, static_cast<long>(a.rows) * a.heads * a.dim, a.key_slices, stream))
       return e;
   if (!need_dkv) return hipSuccess;
-  hipLaunchKernelGGL((attn_dkv_k<T, DP, VEC, DROP>), dim3(shared), dim3(256 * DkvShape<T, DP>::kSplit), 0, stream, a);
+  hipLaunchKernelGGL((attn_dkv_k<T, DP, VEC, DROP>), dim3(shared), dim3(kThreads), 0, stream, a);
   if (hipError_t e = hipGetLastError()) return e;
   if (a.query_slices == 1) return hipSuccess;
   return fold<T>(a.dk, a.dv, a.partial, static_cast<long>(a.rows) * a.kv_heads * a.dim, a.query_slices, stream);
@@ -794,6 +797,24 @@ long bf_attn_partial_floats(const BfAttnArgs* a) {
   const long keys = a->key_slices > 1 ? a->key_slices * wide * (a->dim + 1) : 0;
   const long queries = a->query_slices > 1 ? a->query_slices * narrow * a->dim * 2 : 0;
   return keys > queries ? keys : queries;
+}
+
+// Whether the launches have room for the workgroups of any bounds: fewer than
+// 2^24 tiles and heads together, or 2^23 for dk and dv of wide half-type heads,
+// whose workgroups are twice as large.
+int bf_attn_fits(const BfAttnArgs* a, int dtype, int backward) {
+  if (a->rows == 0) return 1;  // nothing is launched
+  const long tiles = most_tiles(*a, kRows);
+  if (units(tiles * bf_attn_key_slices(a, dtype), a->heads) * 256 > kMostThreads) return 0;
+  const int threads = dtype != 0 && a->dim > 64 ? 512 : 256;
+  return !backward || units(tiles * bf_attn_query_slices(a, dtype), a->kv_heads) * threads <= kMostThreads;
+}
+
+int bf_attn_table_ints(const BfAttnArgs* a) { return a->seqs > kLanes ? a->seqs + 1 : 0; }
+
+hipError_t bf_attn_table(const BfAttnArgs* a, int* table, hipStream_t stream) {
+  hipLaunchKernelGGL(attn_table_k, dim3(1), dim3(1024), 0, stream, *a, table);
+  return hipGetLastError();
 }
 
 hipError_t bf_attn_fwd(const BfAttnArgs* a, int dtype, hipStream_t stream) {

@@ -314,7 +314,8 @@ __device__ __forceinline__ float swap_halves(float x) {
 // The sequences' tiles of `size` rows are numbered through, and so are those
 // of the rows behind the last sequence (`seq` == seqs then). Bounds that are
 // not ordered or leave [0, rows] are cut to it, so that no access leaves the
-// tensors. Every wave searches by itself, a lane to a sequence.
+// tensors. Every wave searches by itself: up to kLanes sequences with a lane to
+// each, more in a table of the call's.
 // ---------------------------------------------------------------------------
 
 struct Unit {
@@ -365,34 +366,83 @@ __device__ __forceinline__ int sum_up_to(int x) {
   return x;
 }
 
+// The table of more than kLanes sequences: tiles in front of each, and of all.
+// Every workgroup would read all bounds otherwise, so that the time grew with the
+// square of their number: 3000 sequences of 0 to 3 tokens (12 heads of 64, bf16,
+// forward and backward) took 1643 us that way and take 658 with the table, 80 of 64
+// tokens 79 and 82.
+constexpr int kLanes = 64;
+
+// x + y; sums of tiles stay at kMostTiles once they reach it
+__device__ __forceinline__ int add_tiles(int x, int y) { return min(x + y, kMostTiles); }
+
+__device__ __forceinline__ int tiles_of(const BfAttnArgs& a, int seq, int size) {
+  const int2 b = bounds_of(a, seq);
+  return min((b.y - b.x + size - 1) / size, kMostTiles);
+}
+
+// table[i] for i in 0 .. seqs, by one workgroup of 16 waves
+__device__ __forceinline__ void make_table(const BfAttnArgs& a, int* table, int size) {
+  __shared__ int sums[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int before = 0;
+  if (threadIdx.x == 0) table[0] = 0;
+  for (int first = 0; first < a.seqs; first += 1024) {
+    const int seq = first + threadIdx.x;
+    int upto = seq < a.seqs ? tiles_of(a, seq, size) : 0;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int y = __shfl_up(upto, off, 64);
+      if (lane >= off) upto = add_tiles(upto, y);
+    }
+    if (lane == 63) sums[wave] = upto;
+    __syncthreads();
+    int all = before;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (i == wave) upto = add_tiles(upto, all);
+      all = add_tiles(all, sums[i]);
+    }
+    if (seq < a.seqs) table[seq + 1] = upto;
+    before = all;
+    __syncthreads();  // sums are free
+  }
+}
+
 // Tile `number`. Causal tiles cost the more the later they are, and an expensive
-// one that starts last keeps the card waiting: up to 64 sequences' tiles are
+// one that starts last keeps the card waiting: up to kLanes sequences' tiles are
 // numbered by their cost, the most expensive first, as their number from the
 // sequence's start (dk and dv: from its end). Other tiles, which cost as their
 // sequence is long, are numbered in order; sorted they took as long.
 __device__ __forceinline__ Work find_tile(const BfAttnArgs& a, int number, int size, bool causal) {
   const int lane = threadIdx.x & 63;
   Work w{};
-  int first = 0, count = a.seqs, chunk = (a.seqs + 63) / 64, mine = 0;
-  const auto tiles_of = [&]() __attribute__((always_inline)) {  // of the lane's `chunk` sequences
-    int sum = 0;
-#pragma unroll 8
-    for (int i = 0; i < chunk; ++i) {  // unguarded, so that the loads go out together
-      const int at = lane * chunk + i;
-      const int2 b = bounds_of(a, first + min(at, count - 1));
-      sum = min(sum + (at < count ? (b.y - b.x + size - 1) / size : 0), kMostTiles);
-    }
-    return sum;
-  };
-  if (count) mine = tiles_of();
-  int upto = sum_up_to(mine);
-  const int all = __builtin_amdgcn_readlane(upto, 63);
+  int mine = 0, upto = 0, all;
+  if (a.seqs > kLanes) {
+    all = a.table[a.seqs];
+  } else {
+    mine = lane < a.seqs ? tiles_of(a, lane, size) : 0;
+    upto = sum_up_to(mine);
+    all = __builtin_amdgcn_readlane(upto, 63);
+  }
   if (number >= all) {  // behind the last sequence
     const int2 rest = bounds_of(a, a.seqs);
     w.seq = a.seqs;
     w.tile = number - all;
     if (w.tile * size >= rest.y - rest.x) return w;
-  } else if (causal && chunk == 1) {
+  } else if (a.seqs > kLanes) {
+    // the last sequence with no more than `number` tiles in front: table[first]
+    // <= number < table[first + count]
+    int first = 0, count = a.seqs;
+    while (count > 1) {
+      const int chunk = (count + 63) / 64, at = lane * chunk;
+      const int pick = __popcll(__ballot(at < count && a.table[first + min(at, count)] <= number)) - 1;
+      first += pick * chunk;
+      count = min(chunk, count - pick * chunk);
+    }
+    w.seq = first;
+    w.tile = number - a.table[first];
+  } else if (causal) {
     int low = 0, high = a.rows / size + 1;  // more tiles than `number` cost `low` or more, and not `high`
     while (high - low > 1) {
       const int mid = (low + high) / 2;
@@ -403,18 +453,8 @@ __device__ __forceinline__ Work find_tile(const BfAttnArgs& a, int number, int s
     w.seq = __ffsll(__ballot(sum_up_to(mine > low ? 1 : 0) > number)) - 1;
     w.tile = low;
   } else {
-    while (true) {
-      const int pick = __ffsll(__ballot(upto > number)) - 1;
-      number -= __builtin_amdgcn_readlane(upto - mine, pick);
-      first += pick * chunk;
-      if (chunk == 1) break;
-      count = min(chunk, count - pick * chunk);
-      chunk = (count + 63) / 64;
-      mine = tiles_of();
-      upto = sum_up_to(mine);
-    }
-    w.seq = first;
-    w.tile = number;
+    w.seq = __ffsll(__ballot(upto > number)) - 1;
+    w.tile = number - __builtin_amdgcn_readlane(upto - mine, w.seq);
   }
   w.seq = __builtin_amdgcn_readfirstlane(w.seq);
   w.tile = __builtin_amdgcn_readfirstlane(w.tile);

@@ -27,6 +27,7 @@ struct BfAttnArgs {
   float* partial;  // bf_attn_partial_floats() of them
   int key_slices, query_slices;  // of the axes that workgroups go along
   const int* cu;  // seqs + 1 ends of the sequences
+  const int* table;  // bf_attn_table_ints() of them, by bf_attn_table
   int seqs, rows, heads, kv_heads, dim;
   // element strides of a row and a head; the last dimension is dense
   long q_row, q_head, k_row, k_head, v_row, v_head, do_row, do_head;
@@ -51,6 +52,9 @@ struct BfNormArgs {
 };
 
 extern "C" {
+int bf_attn_fits(const BfAttnArgs* a, int dtype, int backward);
+int bf_attn_table_ints(const BfAttnArgs* a);
+hipError_t bf_attn_table(const BfAttnArgs* a, int* table, hipStream_t stream);
 hipError_t bf_attn_fwd(const BfAttnArgs* a, int dtype, hipStream_t stream);
 int bf_attn_key_slices(const BfAttnArgs* a, int dtype);
 int bf_attn_query_slices(const BfAttnArgs* a, int dtype);

@@ -115,13 +115,14 @@ Tensor readable(const Tensor& t) {
   return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
-BfAttnArgs attn_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu,
+BfAttnArgs attn_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu, const Tensor& table,
                      double scale, bool causal, const BfDropout& drop) {
   BfAttnArgs a{};
   a.q = q.const_data_ptr();
   a.k = k.const_data_ptr();
   a.v = v.const_data_ptr();
   a.cu = cu.const_data_ptr<int>();
+  a.table = table.defined() ? table.const_data_ptr<int>() : nullptr;
   a.seqs = static_cast<int>(cu.numel()) - 1;
   a.rows = static_cast<int>(q.size(0));
   a.heads = static_cast<int>(q.size(1));
@@ -146,14 +147,21 @@ Tensor attn_partial(BfAttnArgs& a, const at::TensorOptions& f32) {
 }
 
 Tensor attn_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu,
-                    double scale, bool causal, const BfDropout& drop, Tensor* lse, Tensor* rest) {
+                    double scale, bool causal, const BfDropout& drop, Tensor* lse, Tensor* rest, Tensor* kept_table) {
   c10::DeviceGuard guard(q.device());
   Tensor out = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
   if (lse) *lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
   if (rest && q.scalar_type() != at::kFloat) *rest = at::empty(out.sizes(), q.options());
   if (out.numel() == 0) return out;
   with_memory("packed_attention", {&out});  // a mode may make new tensors fake
-  BfAttnArgs a = attn_args(q, k, v, cu, scale, causal, drop);
+  BfAttnArgs a = attn_args(q, k, v, cu, Tensor(), scale, causal, drop);
+  Tensor table;
+  if (const int n = bf_attn_table_ints(&a)) {
+    table = at::empty({n}, cu.options());
+    a.table = table.data_ptr<int>();
+    check(bf_attn_table(&a, table.data_ptr<int>(), stream_of(q)), "packed_attention");
+  }
+  if (kept_table) *kept_table = table;
   a.o = out.data_ptr();
   a.lse = lse ? lse->data_ptr<float>() : nullptr;
   a.rest = rest && rest->defined() ? rest->data_ptr() : nullptr;
@@ -168,10 +176,10 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
                         const Tensor& cu, const std::optional<Tensor>& seed_tensor, double scale,
                         bool causal, double p, int64_t seed, int64_t offset) {
-    Tensor lse, rest;
+    Tensor lse, rest, table;
     const Tensor st = seed_tensor.value_or(Tensor());
-    Tensor out = attn_forward(q, k, v, cu, scale, causal, dropout_args(st, seed, offset, p), &lse, &rest);
-    ctx->save_for_backward({q, k, v, cu, st, out, lse, rest});
+    Tensor out = attn_forward(q, k, v, cu, scale, causal, dropout_args(st, seed, offset, p), &lse, &rest, &table);
+    ctx->save_for_backward({q, k, v, cu, st, out, lse, rest, table});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["p"] = p;
@@ -185,8 +193,8 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
     variable_list none(10);
     if (!grads[0].defined()) return none;
     const variable_list s = ctx->get_saved_variables();
-    const Tensor &q = s[0], &k = s[1], &v = s[2], &cu = s[3], &seed_tensor = s[4], &out = s[5], &lse = s[6], &rest = s[7];
-    with_memory("packed_attention backward", {&q, &k, &v, &cu, &seed_tensor, &out, &lse, &rest, &grads[0]});
+    const Tensor &q = s[0], &k = s[1], &v = s[2], &cu = s[3], &seed_tensor = s[4], &out = s[5], &lse = s[6], &rest = s[7], &table = s[8];
+    with_memory("packed_attention backward", {&q, &k, &v, &cu, &seed_tensor, &out, &lse, &rest, &table, &grads[0]});
     c10::DeviceGuard guard(q.device());
     const bool need_dq = ctx->needs_input_grad(0);
     const bool need_dkv = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
@@ -197,7 +205,7 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
     with_memory("packed_attention backward", {&dq});
     if (out.numel()) {
       Tensor delta = at::empty(lse.sizes(), lse.options());
-      BfAttnArgs a = attn_args(q, k, v, cu, ctx->saved_data["scale"].toDouble(),
+      BfAttnArgs a = attn_args(q, k, v, cu, table, ctx->saved_data["scale"].toDouble(),
                                ctx->saved_data["causal"].toBool(),
                                dropout_args(seed_tensor, ctx->saved_data["seed"].toInt(),
                                             ctx->saved_data["offset"].toInt(),
@@ -241,13 +249,18 @@ Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
   TORCH_CHECK_VALUE(cu.numel() <= 1 << 24, "too many sequences");
   TORCH_CHECK_VALUE(scale > 0 && std::isfinite(scale), "scale has to be positive and finite, got ", scale);
   check_dropout(q, st, offset, p);
-  code_of(q);
+  const int code = code_of(q);
+  const bool grad = any_grad({&q, &k, &v});
+  BfAttnArgs size{};
+  size.seqs = static_cast<int>(cu.numel()) - 1, size.rows = static_cast<int>(q.size(0)), size.dim = static_cast<int>(q.size(2));
+  size.heads = static_cast<int>(q.size(1)), size.kv_heads = static_cast<int>(k.size(1));
+  TORCH_CHECK_VALUE(bf_attn_fits(&size, code, grad), "too many sequences or tokens for ", q.size(1), " heads: ", cu.numel() - 1,
+                    " sequences, ", q.size(0), " tokens");
   with_memory("packed_attention", {&q, &k, &v, &cu, &st});
   no_tangents("packed_attention", {&q, &k, &v});
-  const bool grad = any_grad({&q, &k, &v});
   const Tensor rq = readable(q), rk = readable(k), rv = readable(v);
   if (grad) return PackedAttention::apply(rq, rk, rv, cu, seed_tensor, scale, causal, p, seed, offset);
-  return attn_forward(rq, rk, rv, cu, scale, causal, dropout_args(st, seed, offset, p), nullptr, nullptr);
+  return attn_forward(rq, rk, rv, cu, scale, causal, dropout_args(st, seed, offset, p), nullptr, nullptr, nullptr);
 }
 
 // ---------------------------------------------------------------------------

@@ -64,6 +64,9 @@ def packed_attention(
     ``cu_seqlens[b + 1]``; ``cu_seqlens`` is int32 on the same device, starts
     with 0 and does not decrease (a GPU kernel cannot raise on its values: it
     only guarantees to stay inside the tensors). Empty sequences are allowed.
+    A GPU call has room for fewer than 2**24 / heads tiles, of which a sequence
+    takes one to every 128 tokens or part of them (2**23 / kv_heads if gradients
+    are needed of half types with dim above 64).
     Rows behind the last sequence give zeros and take no part, whatever they
     hold; their gradients are zero.
 

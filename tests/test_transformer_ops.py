@@ -1044,3 +1044,54 @@ def test_mapped_over_a_dimension():
     a, b = (torch.autograd.grad(y.sum(), w)[0] for y in (got, want))
     # sums of 12 terms of size below 8 in another order
     assert (a - b).abs().max() <= 2 * 12 * 12 * 8 * F32
+
+
+# ---------------------------------------------------------------------------
+# many sequences
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_many_sequences(device, dtype, causal):
+    """Over a thousand, some of several tiles, empty ones among them."""
+    g = torch.Generator().manual_seed(6)
+    lengths = torch.tensor([0, 0, 1, 2, 3, 17, 140])[torch.randint(0, 7, (1100,), generator=g)].tolist()
+    lengths[500] = 300
+    attention_agrees(device, dtype, lengths, 12, 4, 16, causal=causal, spare=150)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_very_many_sequences(causal):
+    """2**17 of one token: the output is v, and the gradients are 0 and dO."""
+    n = 1 << 17
+    q, k, v, dout = attention_inputs((n,), 12, 12, 8, torch.float16, "cuda")
+    cu = torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    got = attention(q, k, v, dout, cu, causal=causal)
+    assert torch.equal(got["out"], v) and torch.equal(got["dv"], dout)
+    assert not got["dq"].any() and not got["dk"].any()
+
+
+def test_attention_refuses_more_tiles_than_a_launch_holds():
+    """Before the forward pass, also where only the backward pass has no room
+    for them. Fake tensors: nothing is launched."""
+    from torch._subclasses import FakeTensorMode
+
+    if not hip_ext.has_extension():
+        pytest.skip("the native extension is not built")
+    with FakeTensorMode():
+        def call(sequences, heads, dim, dtype, needs=False, tokens=8):
+            q = torch.empty(tokens, heads, dim, dtype=dtype, device="cuda", requires_grad=needs)
+            bf.packed_attention(q, q, q, torch.empty(sequences + 1, dtype=torch.int32, device="cuda"))
+
+        refused(ValueError, "too many", call, 1 << 23, 2, 64, torch.float32)
+        refused(ValueError, "too many", call, 1 << 18, 64, 64, torch.bfloat16)
+        refused(ValueError, "too many", call, 1 << 23, 1, 128, torch.bfloat16, True)
+        refused(ValueError, "too many", call, 0, 128, 8, torch.float16, tokens=1 << 24)
+        # these have room: they reach the next refusal
+        refused(NotImplementedError, "memory", call, 1 << 23, 1, 128, torch.bfloat16)
+        refused(NotImplementedError, "memory", call, 1 << 23, 1, 128, torch.float32, True)
+        refused(NotImplementedError, "memory", call, (1 << 24) - 9, 1, 64, torch.float16, True)
+        refused(NotImplementedError, "memory", call, (1 << 24) - 1, 65535, 64, torch.float16, tokens=0)
