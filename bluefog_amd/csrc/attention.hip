@@ -613,7 +613,9 @@ __attribute__((amdgpu_waves_per_eu(DkvShape<T, DP>::kWaves, DkvShape<T, DP>::kWa
           }
           bits <<= 4 * half;
           bits |= __float_as_uint(swap_halves(__uint_as_float(bits)));
+          wave_exchange();  // the last mask is read
           if (half == 0) kept[wave][lane] = bits;
+          wave_exchange();
         }
         float p[16], ds[16];
 #pragma unroll

@@ -223,6 +223,15 @@ __device__ __forceinline__ void loads_done() {
   __syncthreads();
 }
 
+// LDS that the lanes of one wave exchange: what stands in front is done before
+// what follows. The hardware keeps a wave's LDS accesses in order; this tells the
+// compiler, at no instruction.
+__device__ __forceinline__ void wave_exchange() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // The order of a stretch of matrix products and the LDS reads that feed them:
 // AHEAD reads first, then a product and EACH reads in turn. Left to itself the
 // compiler reads one fragment at a time and waits for it, four times as long as
