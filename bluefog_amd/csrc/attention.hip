@@ -110,7 +110,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kFwdWaves<T
   const float c = a.scale * kLog2e;
   float m = -INFINITY, l = 0.f;  // of scores without c
   // One tile of keys, the first 32 * SUBS of them. MASKED: some of them are not
-  // seen by some of the workgroup's rows. CLEAN: see below.
+  // seen by some of the workgroup's rows. CLEAN: v that is no number or infinite
+  // is left out.
   const auto attend = [&](auto mode, auto subs, int k0, int buf) __attribute__((always_inline)) {
     constexpr bool MASKED = decltype(mode)::value > 0, CLEAN = decltype(mode)::value > 1;
     constexpr int SUBS = decltype(subs)::value;
@@ -166,30 +167,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kFwdWaves<T
         for (int i = 0; i < kDT; ++i) o[i] = mma(KV::read_columns(lds[buf][1], columns, u * 16, i), p[u], o[i]);
     } else {
 #pragma unroll
-      for (int i = 0; i < kDT; ++i) {
-        Acc count{};
+      for (int u = 0; u < 2 * SUBS; ++u)
 #pragma unroll
-        for (int u = 0; u < 2 * SUBS; ++u) {
-          Frag<T> f = KV::read_columns(lds[buf][1], columns, u * 16, i), bad, sees;
+        for (int i = 0; i < kDT; ++i) {
+          Frag<T> f = KV::read_columns(lds[buf][1], columns, u * 16, i);
 #pragma unroll
-          for (int r = 0; r < 8; ++r) {
-            const bool fine = fabsf(static_cast<float>(f[r])) < INFINITY;
-            bad[r] = static_cast<T>(fine ? 0.f : 1.f);
-            f[r] = fine ? f[r] : static_cast<T>(0.f);
-            sees[r] = static_cast<T>(k0 + u * 16 + row_of(r, half) < seen ? 1.f : 0.f);
-          }
+          for (int r = 0; r < 8; ++r) f[r] = finite(f[r]) ? f[r] : static_cast<T>(0.f);
           o[i] = mma(f, p[u], o[i]);
-          count = mma(bad, sees, count);
         }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[i][r] = count[r] > 0.f ? NAN : o[i][r];
-      }
     }
   };
   // all tiles, from the one whose load is under way into buffer 0; those that
   // no row has to mask have a loop of their own
   const auto all_tiles = [&](auto masked) __attribute__((always_inline)) {
-    const int whole = min(range.y, (a.causal ? q0 + 1 : w.len) / BN * BN);
+    constexpr bool kClean = decltype(masked)::value > 1;
+    const int whole = kClean ? range.x : min(range.y, (a.causal ? q0 + 1 : w.len) / BN * BN);
     loads_done();
     int k0 = range.x, buf = 0;
     const auto next = [&]() __attribute__((always_inline)) {
@@ -213,23 +205,65 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kFwdWaves<T
     }
   };
   all_tiles(Mode<1>());
-  if (a.causal) {
-    // A masked P is 0, and 0 times a value that is no number is none: if a v
-    // of the masked tiles holds one, rows that do not see it have lost their
-    // sum. Once more then, and it leaves the product: its column is set for the
-    // rows that see the key.
-    bool lost = false;
+  // A P of 0 times a v that is no number or infinite is no number. That P may be
+  // masked, or of a row behind the sequence (which repeats the last), or have been
+  // rounded to 0 where the sum has an infinity. So if a sum is lost, once more
+  // without such v, which are then added where the row sees the key: as they are with
+  // a P, and no number with a P of 0 (a score of -inf, or dropped).
+  bool lost = false;
 #pragma unroll
-    for (int i = 0; i < kDT; ++i)
+  for (int i = 0; i < kDT; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) lost |= !(fabsf(o[i][r]) < INFINITY);
-    if (__syncthreads_or(lost)) {
-      m = -INFINITY, l = 0.f;
+    for (int r = 0; r < 16; ++r) lost |= !finite(o[i][r]);
+  if (__syncthreads_or(lost)) {
+    m = -INFINITY, l = 0.f;
 #pragma unroll
-      for (int i = 0; i < kDT; ++i) o[i] = Acc{};
-      k.load(lds[0][0], range.x, last);
-      v.load(lds[0][1], range.x, last);
-      all_tiles(Mode<2>());
+    for (int i = 0; i < kDT; ++i) o[i] = Acc{};
+    k.load(lds[0][0], range.x, last);
+    v.load(lds[0][1], range.x, last);
+    all_tiles(Mode<2>());
+    for (int k0 = range.x; k0 < range.y; k0 += 32) {  // half a tile's rows, in buffer 0
+      const int at = (k0 - range.x) % BN;
+      if (at == 0) {
+        k.load(lds[0][0], k0, last);
+        v.load(lds[0][1], k0, last);
+        loads_done();
+      }
+      bool bad = false;  // the lane's key has such a v
+      if (lane < 32)
+        for (int d = 0; d < DP; ++d) bad |= !finite(KV::value(lds[0][1], at + lane, d));
+      uint32_t left = static_cast<uint32_t>(__ballot(bad));
+      if (left) {
+        const int rows = KV::row_place(lane & 31, half);
+        Acc s{};
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) s = mma(KV::read_row(lds[0][0], rows, at, i, half), qf[i], s);
+        uint32_t with = 0, without = 0;  // keys that the row sees, by their P
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          uint4 bits;
+          if (DROP) bits = bf_philox((k0 / 16 + t) * 2 + half, static_cast<uint32_t>(row), h, a.drop.offset, key);
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            const int j = t * 16 + row_of(r, half);
+            const bool keep = !DROP || bf_half(bits, r) >= a.drop.threshold;
+            if (k0 + j < seen) (keep && s[t * 8 + r] > -INFINITY ? with : without) |= 1u << j;
+          }
+        }
+        with |= __float_as_uint(swap_halves(__uint_as_float(with)));
+        without |= __float_as_uint(swap_halves(__uint_as_float(without)));
+        for (; left; left &= left - 1) {
+          const int j = __builtin_ctz(left), h2 = here<true>(half);
+#pragma unroll
+          for (int i = 0; i < kDT; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const T x = KV::value(lds[0][1], at + j, i * 32 + row_of(r, h2));
+              if (!finite(x)) o[i][r] += with >> j & 1 ? static_cast<float>(x) : without >> j & 1 ? NAN : 0.f;
+            }
+        }
+      }
+      if (at + 32 == BN) __syncthreads();  // the buffer is free
     }
   }
   l += swap_halves(l);
@@ -260,7 +294,7 @@ __global__ __launch_bounds__(256) void attn_join_k(BfAttnArgs a) {
       for (int u = 0; u < 4; ++u) x[u] = u < n ? part[u] : 0.f;
     total += share;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) out[u] += share * x[u];
+    for (int u = 0; u < 4; ++u) out[u] += fabsf(x[u]) < INFINITY ? share * x[u] : x[u];  // a share may round to 0
   }
   T* o = static_cast<T*>(a.o) + at * a.dim + c;
   T* rest = a.rest ? static_cast<T*>(a.rest) + at * a.dim + c : nullptr;

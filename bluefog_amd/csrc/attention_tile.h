@@ -52,6 +52,9 @@ __device__ __forceinline__ Frag<T> rest_of(const float* x, Frag<T> of) {
   return rounded<T>(less);
 }
 
+template <typename T>
+__device__ __forceinline__ bool finite(T x) { return fabsf(static_cast<float>(x)) < INFINITY; }
+
 __device__ __forceinline__ Acc mma(Frag<__bf16> a, Frag<__bf16> b, Acc c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
@@ -99,6 +102,10 @@ struct Tile {
 
   static __device__ __forceinline__ void clear(char* lds, int bytes) {
     for (int i = threadIdx.x * 16; i < bytes; i += THREADS * 16) *reinterpret_cast<uint4*>(lds + i) = uint4{0, 0, 0, 0};
+  }
+
+  static __device__ __forceinline__ T value(const char* lds, int row, int column) {
+    return *reinterpret_cast<const T*>(lds + at(row, column / kEach) + column % kEach * sizeof(T));
   }
 
   // Places of a lane in a tile, from which those of its fragments differ in bits

@@ -124,7 +124,13 @@ def packed_attention(
         prob = torch.softmax(score, 2)
         if dropout_p:
             prob = _masked(prob, _attention_bits(heads, begin, n, key, offset, q.device), dropout_p)
-        parts.append(torch.matmul(prob, sv).transpose(0, 1).to(q.dtype))
+        if causal and not torch.isfinite(sv).all():
+            # a masked probability of 0 times such a value would be no number
+            out = [torch.matmul(prob[:, i : i + 1, : i + 1], sv[:, : i + 1]) for i in range(n)]
+            out = torch.cat(out, 1)
+        else:
+            out = torch.matmul(prob, sv)
+        parts.append(out.transpose(0, 1).to(q.dtype))
     # zeros behind the last sequence, tied to the inputs for the case that no
     # sequence has a row
     rest = q[ends[-1]:].masked_fill(torch.ones((), dtype=torch.bool, device=q.device), 0.0)

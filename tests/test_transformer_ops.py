@@ -1095,3 +1095,90 @@ def test_attention_refuses_more_tiles_than_a_launch_holds():
         refused(NotImplementedError, "memory", call, 1 << 23, 1, 128, torch.float32, True)
         refused(NotImplementedError, "memory", call, (1 << 24) - 9, 1, 64, torch.float16, True)
         refused(NotImplementedError, "memory", call, (1 << 24) - 1, 65535, 64, torch.float16, tokens=0)
+
+
+# ---------------------------------------------------------------------------
+# values that are infinite or no number
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dim", [40, 64, 128, 57])
+@pytest.mark.parametrize("p", [0.0, 0.3])
+def test_attention_infinite_values(device, dtype, causal, dim, p):
+    """An infinite v is infinite in every row that sees its key with a
+    probability above 0, wherever the key lies; no number if the probability is
+    dropped or another such v is of the other sign; nothing to rows that do not
+    see it, and to other columns. The rest keeps its bits on the GPU, where the
+    sums are the same; on the CPU it has the roundings of a sum of n terms."""
+    if device == "cpu" and dim != 40:
+        pytest.skip("the torch code does not depend on the head size")
+    n = 700 if device == "cuda" else 70
+    for lengths, bad in [((150, 40), [(140, 3, math.inf), (149, 5, -math.inf), (160, 7, math.inf)]),
+                         ((150, 40), [(2, 0, math.inf), (70, 0, -math.inf), (189, 6, -math.inf), (100, 1, math.nan)]),
+                         ((n,), [(n - 10, 1, math.inf), (31, 2, -math.inf), (n - 1, 4, math.inf)])]:
+        q, k, v, _ = attention_inputs(lengths, 2, 1, dim, dtype, device)
+        cu, kw = ends_of(lengths, device), dict(causal=causal, dropout_p=p, seed=3)
+        with torch.no_grad():
+            clean_v = v.detach().clone()
+            for row, column, value in bad:
+                v[row, 0, column], clean_v[row, 0, column] = value, 0
+            clean = bf.packed_attention(q, k, clean_v, cu, **kw).cpu()
+            got = bf.packed_attention(q, k, v, cu, **kw).cpu()
+        want = clean.double()
+        ends = cu.tolist()
+        for row, column, value in bad:
+            begin, end = next((a, b) for a, b in zip(ends, ends[1:]) if a <= row < b)
+            keep = attention_keep(2, begin, end - begin, p, 3, 0)[:, :, row - begin] > 0
+            for i in range(row if causal else begin, end):
+                for h in range(2):
+                    want[i, h, column] += value if keep[h, i - begin] else math.nan
+        fine = torch.isfinite(want)
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        assert torch.equal(got[~fine].double().nan_to_num(7.0), want[~fine].nan_to_num(7.0))
+        off = (got.double() - want)[fine].abs()
+        if device == "cuda":
+            assert not off.any()
+        else:
+            size = v[torch.isfinite(v)].abs().max().item() / (1 - p)
+            assert (off <= 2 * (max(lengths) + 16) * F32 * size + 2 * rounding(dtype, want[fine])).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_infinite_value_of_small_probability(device, dtype, causal):
+    """A probability of e**-25, which f16 does not hold, is above 0; one whose score
+    is -inf is 0."""
+    n = 90
+    q, k, v, _ = (t.detach() for t in attention_inputs((n,), 1, 1, 64, dtype, device))
+    q[:, 0, 0], k[:, 0, 0], k[4, 0] = 20.0, 0.0, 0.0
+    k[4, 0, 0] = -10.0  # the score of key 4: -200 / 8; the others' are of size 1
+    v[4, 0, 9] = math.inf
+    got = bf.packed_attention(q, k, v, ends_of((n,), device), causal=causal)
+    first = 4 if causal else 0
+    assert (got[first:, 0, 9] == math.inf).all() and torch.isfinite(got[:first]).all()
+    k[4, 0, 0] = -math.inf
+    got = bf.packed_attention(q, k, v, ends_of((n,), device), causal=causal)
+    assert torch.isnan(got[first:, 0, 9]).all() and torch.isfinite(got[:first]).all()
+    assert torch.isfinite(got[first:, 0, :9]).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_attention_causal_rows_ignore_later_values(device, dtype, bad):
+    """A later key or value that is not a number leaves earlier rows alone, on the
+    CPU too; there the last bits may differ, since rows are summed one by one."""
+    for n, at in ((50, 37), (300, 150)):
+        q, k, v, _ = (t.detach() for t in attention_inputs((n,), 2, 2, 64, dtype, device))
+        cu = ends_of((n,), device)
+        clean = bf.packed_attention(q, k, v, cu, causal=True)
+        size = v.abs().max().item()
+        k[at], v[at] = bad, bad
+        got = bf.packed_attention(q, k, v, cu, causal=True)
+        off = (got[:at].cpu().double() - clean[:at].cpu().double()).abs()
+        assert (off <= 2 * (n + 16) * F32 * size + 2 * rounding(dtype, clean[:at].cpu().double())).all()
+        assert not torch.isfinite(got[at:]).any()
