@@ -16,8 +16,3 @@ template <>
 __device__ __forceinline__ float bf_to_float(_Float16 x) { return static_cast<float>(x); }
 template <>
 __device__ __forceinline__ float bf_to_float(__bf16 x) { return static_cast<float>(x); }
-
-template <typename T, int N>
-struct alignas(sizeof(T) * N) BfPack {
-  T v[N];
-};

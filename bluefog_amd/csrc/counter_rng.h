@@ -10,6 +10,11 @@
 // if its value is at least `threshold` = round(65536 p), so p is held to 16
 // bits and the kept elements are scaled by 65536 / (65536 - threshold), which
 // keeps the expectation exact for the probability that is really used.
+//
+// Attention: the keys of sixteen share two calls by quads, 0-3 and 8-11, and 4-7
+// and 12-15, which is how a 32x32 matrix tile spreads them over lanes: key j of
+// (head, packed query row) takes value ((j >> 3) & 1) * 4 + (j & 3) of the call with
+// counter ((j >> 4) * 2 + ((j >> 2) & 1), row, head, offset).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -60,23 +65,4 @@ __device__ __forceinline__ uint4 bf_flat_bits(uint64_t block,
                                               const BfDropout& d, BfKey k) {
   return bf_philox(static_cast<uint32_t>(block),
                    static_cast<uint32_t>(block >> 32), 0u, d.offset, k);
-}
-
-// factor of element i of a tensor: 0, or the scale of what is kept
-__device__ __forceinline__ float bf_flat_keep(uint64_t i, const BfDropout& d,
-                                              BfKey k) {
-  const uint4 w = bf_flat_bits(i >> 3, d, k);
-  return bf_half(w, static_cast<int>(i & 7)) >= d.threshold ? d.scale : 0.f;
-}
-
-// Attention: the probability of (head, packed query row, key j of the row's
-// sequence). The keys of sixteen share two calls by quads: 0-3 and 8-11, and
-// 4-7 and 12-15, which is how a 32x32 matrix tile spreads them over lanes.
-__device__ __forceinline__ float bf_attn_keep(uint32_t head, uint32_t row,
-                                              uint32_t j, const BfDropout& d,
-                                              BfKey k) {
-  const uint4 w =
-      bf_philox((j >> 4) * 2 + ((j >> 2) & 1), row, head, d.offset, k);
-  const int u = static_cast<int>(((j >> 3) & 1) * 4 + (j & 3));
-  return bf_half(w, u) >= d.threshold ? d.scale : 0.f;
 }

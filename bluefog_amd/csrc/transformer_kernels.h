@@ -59,8 +59,8 @@ hipError_t bf_attn_fwd(const BfAttnArgs* a, int dtype, hipStream_t stream);
 int bf_attn_key_slices(const BfAttnArgs* a, int dtype);
 int bf_attn_query_slices(const BfAttnArgs* a, int dtype);
 long bf_attn_partial_floats(const BfAttnArgs* a);
-hipError_t bf_attn_bwd(const BfAttnArgs* a, int dtype, int need_dq,
-                       int need_dkv, hipStream_t stream);
+// dq always: delta, which dk and dv need, comes with it
+hipError_t bf_attn_bwd(const BfAttnArgs* a, int dtype, int need_dkv, hipStream_t stream);
 hipError_t bf_norm_fwd(const BfNormArgs* a, int x_dtype, int r_dtype,
                        hipStream_t stream);
 hipError_t bf_norm_bwd(const BfNormArgs* a, int x_dtype, int r_dtype,

@@ -196,7 +196,6 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
     const Tensor &q = s[0], &k = s[1], &v = s[2], &cu = s[3], &seed_tensor = s[4], &out = s[5], &lse = s[6], &rest = s[7], &table = s[8];
     with_memory("packed_attention backward", {&q, &k, &v, &cu, &seed_tensor, &out, &lse, &rest, &table, &grads[0]});
     c10::DeviceGuard guard(q.device());
-    const bool need_dq = ctx->needs_input_grad(0);
     const bool need_dkv = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
     const Tensor dout = readable(grads[0]);
     Tensor dq = at::empty(out.sizes(), out.options());
@@ -222,7 +221,7 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
       a.key_slices = bf_attn_key_slices(&a, code_of(q));
       a.query_slices = need_dkv ? bf_attn_query_slices(&a, code_of(q)) : 1;
       const Tensor partial = attn_partial(a, lse.options());
-      check(bf_attn_bwd(&a, code_of(q), need_dq, need_dkv, stream_of(q)), "packed_attention backward");
+      check(bf_attn_bwd(&a, code_of(q), need_dkv, stream_of(q)), "packed_attention backward");
     }
     none[0] = dq, none[1] = dk, none[2] = dv;
     return none;
@@ -284,7 +283,7 @@ std::pair<Tensor, int64_t> as_rows(const Tensor& t) {
   return {t.contiguous(), width};
 }
 
-BfNormArgs norm_args(const Tensor& x, const Tensor& r, const Tensor& weight, const Tensor& bias,
+BfNormArgs norm_args(const Tensor& x, const Tensor& weight, const Tensor& bias,
                      double eps, const BfDropout& drop) {
   BfNormArgs a{};
   a.width = static_cast<int>(x.size(-1));
@@ -303,7 +302,7 @@ Tensor norm_forward(const Tensor& x, const Tensor& r, const Tensor& weight, cons
   c10::DeviceGuard guard(x.device());
   const Tensor& kind = r.defined() ? r : x;
   Tensor y = at::empty(x.sizes(), kind.options(), at::MemoryFormat::Contiguous);
-  BfNormArgs a = norm_args(x, r, weight, bias, eps, drop);
+  BfNormArgs a = norm_args(x, weight, bias, eps, drop);
   if (mean) {
     *mean = at::empty({a.rows}, x.options().dtype(at::kFloat));
     *rstd = at::empty({a.rows}, x.options().dtype(at::kFloat));
@@ -352,7 +351,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const Tensor &x = s[0], &r = s[1], &weight = s[2], &bias = s[3], &seed_tensor = s[4];
     with_memory("layer_norm backward", {&x, &r, &weight, &bias, &seed_tensor, &s[5], &s[6], &grads[0]});
     c10::DeviceGuard guard(x.device());
-    BfNormArgs a = norm_args(x, r, weight, bias, ctx->saved_data["eps"].toDouble(),
+    BfNormArgs a = norm_args(x, weight, bias, ctx->saved_data["eps"].toDouble(),
                              dropout_args(seed_tensor, ctx->saved_data["seed"].toInt(),
                                           ctx->saved_data["offset"].toInt(), ctx->saved_data["p"].toDouble()));
     const Tensor& kind = r.defined() ? r : x;
