@@ -246,7 +246,8 @@ Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
   TORCH_CHECK_TYPE(cu.scalar_type() == at::kInt, "cu_seqlens has to be int32");
   TORCH_CHECK_VALUE(cu.dim() == 1 && cu.numel() >= 1 && cu.is_contiguous(), "cu_seqlens has to be a dense vector");
   TORCH_CHECK_VALUE(cu.numel() <= 1 << 24, "too many sequences");
-  TORCH_CHECK_VALUE(scale > 0 && std::isfinite(scale), "scale has to be positive and finite, got ", scale);
+  TORCH_CHECK_VALUE(static_cast<float>(scale) > 0 && std::isfinite(static_cast<float>(scale)),
+                    "scale has to be positive and finite in 32 bits, got ", scale);
   check_dropout(q, st, offset, p);
   const int code = code_of(q);
   const bool grad = any_grad({&q, &k, &v});
@@ -421,7 +422,8 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const st
     TORCH_CHECK_TYPE(r.scalar_type() == at::kFloat || r.scalar_type() == x.scalar_type(),
                      "residual has to be f32 or of the input's type");
   }
-  TORCH_CHECK_VALUE(eps >= 0 && std::isfinite(eps), "eps has to be finite and not negative, got ", eps);
+  TORCH_CHECK_VALUE((eps == 0 || static_cast<float>(eps) > 0) && std::isfinite(static_cast<float>(eps)),
+                    "eps has to be finite and not negative, in 32 bits, got ", eps);
   check_dropout(x, st, offset, p);
   with_memory("layer_norm", {&x, &r, &w, &b, &st});
   no_tangents("layer_norm", {&x, &r, &w, &b});

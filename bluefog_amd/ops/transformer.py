@@ -98,8 +98,9 @@ def packed_attention(
         raise ValueError("cu_seqlens has to be a dense vector on the same device")
     if cu_seqlens.numel() > 1 << 24:
         raise ValueError("too many sequences")
-    if not (scale > 0 and math.isfinite(scale)):
-        raise ValueError(f"scale has to be positive and finite, got {scale}")
+    kept = _held(scale, q.dtype)
+    if not (kept > 0 and math.isfinite(kept)):
+        raise ValueError(f"scale has to be positive and finite in 32 bits, got {scale}")
     ends = cu_seqlens.tolist()
     if ends[0] != 0 or ends[-1] > q.shape[0] or any(a > b for a, b in zip(ends, ends[1:])):
         raise ValueError("cu_seqlens has to rise from 0 to at most the number of tokens")
@@ -180,8 +181,9 @@ def layer_norm(
             raise ValueError("residual has to have the input's shape")
         if residual.dtype not in (torch.float32, x.dtype):
             raise TypeError("residual has to be f32 or of the input's type")
-    if not (eps >= 0 and math.isfinite(eps)):
-        raise ValueError(f"eps has to be finite and not negative, got {eps}")
+    kept = _held(eps, x.dtype)
+    if not ((eps == 0 or kept > 0) and math.isfinite(kept)):
+        raise ValueError(f"eps has to be finite and not negative, in 32 bits, got {eps}")
     seed, value = _seed(seed, x, dropout_p)
     wide = x.dtype if x.dtype == torch.float64 else torch.float32
     z = x.to(wide)
@@ -234,6 +236,12 @@ def _seed(seed: Seed, like: torch.Tensor, p: float):
     if not -(1 << 63) <= seed < 1 << 63:
         raise ValueError(f"seed has to fit 64 bits, got {seed}")
     return None, seed
+
+
+def _held(value: float, dtype: torch.dtype) -> float:
+    """A number as the sums of this type hold it."""
+    wide = torch.float64 if dtype == torch.float64 else torch.float32
+    return torch.tensor(value, dtype=wide).item()
 
 
 def _check(x: torch.Tensor, p: float, offset: int) -> None:

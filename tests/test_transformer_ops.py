@@ -1182,3 +1182,18 @@ def test_attention_causal_rows_ignore_later_values(device, dtype, bad):
         off = (got[:at].cpu().double() - clean[:at].cpu().double()).abs()
         assert (off <= 2 * (n + 16) * F32 * size + 2 * rounding(dtype, clean[:at].cpu().double())).all()
         assert not torch.isfinite(got[at:]).any()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_numbers_that_leave_32_bits_are_refused(device):
+    """A scale or an eps that is 0 or infinite as the kernels hold it."""
+    q, k, v, _ = attention_inputs((8,), 1, 1, 16, torch.float32, device)
+    cu, x = ends_of((8,), device), torch.ones(3, 16, device=device)
+    for scale in (1e-60, 1e39):
+        refused(ValueError, "scale", bf.packed_attention, q, k, v, cu, scale=scale)
+    for eps in (1e-60, 1e39):
+        refused(ValueError, "eps", bf.layer_norm, x, eps=eps)
+    if device == "cpu":  # 64-bit tensors hold them
+        wide = [t.double() for t in (q, k, v)]
+        assert torch.isfinite(bf.packed_attention(*wide, cu, scale=1e-60)).all()
+        assert not bf.layer_norm(x.double(), eps=1e-60).any()
