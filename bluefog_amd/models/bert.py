@@ -6,7 +6,9 @@ ROCm lowers to the MIOpen/CK flash-attention path.
 
 A batch can also be packed: its sequences one behind the other, without
 padding, and ``cu_seqlens`` with their ends. Attention, norms and dropout then
-run in bluefog_amd's own operators (ops/transformer.py)."""
+run in bluefog_amd's own operators (ops/transformer.py), from the same modules:
+each is called, with its own mode and probability, but for the ``nn.Dropout``,
+whose masks the operators draw."""
 
 
 
@@ -41,19 +43,30 @@ class BertConfig:
         self.dropout = dropout
 
 
+def _rate(dropout):
+    """What a dropout module drops in its present mode."""
+    if not isinstance(dropout, (nn.Dropout, nn.Identity)):
+        raise TypeError(f"a packed batch takes nn.Dropout or nn.Identity, not {type(dropout).__name__}")
+    return dropout.p if dropout.training and isinstance(dropout, nn.Dropout) else 0.0
+
+
 class BertEmbeddings(nn.Module):
     def __init__(self, cfg: BertConfig):
         super().__init__()
+        from bluefog_amd.ops.fused_modules import FusedAddLayerNorm
+
         self.word = nn.Embedding(cfg.vocab_size, cfg.hidden_size)
         self.position = nn.Embedding(cfg.max_position_embeddings, cfg.hidden_size)
         self.token_type = nn.Embedding(cfg.type_vocab_size, cfg.hidden_size)
-        self.norm = nn.LayerNorm(cfg.hidden_size, eps=cfg.layer_norm_eps)
+        self.norm = FusedAddLayerNorm(cfg.hidden_size, eps=cfg.layer_norm_eps)
         self.dropout = nn.Dropout(cfg.dropout)
         self.register_buffer(
             "pos_ids", torch.arange(cfg.max_position_embeddings).unsqueeze(0), persistent=False
         )
 
-    def forward(self, input_ids):
+    def forward(self, input_ids, cu_seqlens=None, seed=None):
+        if cu_seqlens is not None:
+            return self._packed(input_ids, cu_seqlens, seed)
         s = input_ids.shape[1]
         x = (
             self.word(input_ids)
@@ -62,8 +75,8 @@ class BertEmbeddings(nn.Module):
         )
         return self.dropout(self.norm(x))
 
-    def packed(self, input_ids, cu_seqlens, p, seed):
-        from bluefog_amd.ops.transformer import counter_dropout, layer_norm
+    def _packed(self, input_ids, cu_seqlens, seed):
+        from bluefog_amd.ops.transformer import counter_dropout
 
         token = torch.arange(input_ids.shape[0], device=input_ids.device, dtype=cu_seqlens.dtype)
         sequence = torch.searchsorted(cu_seqlens, token, right=True) - 1
@@ -71,7 +84,7 @@ class BertEmbeddings(nn.Module):
         # bounds on the GPU are not checked
         pos = (token - cu_seqlens[sequence]).clamp(0, self.position.num_embeddings - 1)
         x = self.word(input_ids) + self.position(pos) + self.token_type(torch.zeros_like(input_ids))
-        x = layer_norm(x, self.norm.weight, self.norm.bias, self.norm.eps)
+        x, p = self.norm(x, None, (0.0, None, 0)), _rate(self.dropout)
         return counter_dropout(x, p, seed) if p else x
 
 
@@ -84,7 +97,9 @@ class BertSelfAttention(nn.Module):
         self.out = nn.Linear(cfg.hidden_size, cfg.hidden_size)
         self.dropout_p = cfg.dropout
 
-    def forward(self, x):
+    def forward(self, x, cu_seqlens=None, seed=None, offset=0):
+        if cu_seqlens is not None:
+            return self._packed(x, cu_seqlens, seed, offset)
         B, S, H = x.shape
         qkv = self.qkv(x).reshape(B, S, 3, self.nh, self.hd).permute(2, 0, 3, 1, 4)
         q, k, v = qkv[0], qkv[1], qkv[2]
@@ -93,9 +108,10 @@ class BertSelfAttention(nn.Module):
         )
         return self.out(o.transpose(1, 2).reshape(B, S, H))
 
-    def packed(self, x, cu_seqlens, p, seed, offset):
+    def _packed(self, x, cu_seqlens, seed, offset):
         from bluefog_amd.ops.transformer import packed_attention
 
+        p = self.dropout_p if self.training else 0.0
         q, k, v = self.qkv(x).view(x.shape[0], 3, self.nh, self.hd).unbind(1)
         o = packed_attention(q, k, v, cu_seqlens, dropout_p=p, seed=seed, offset=offset)
         return self.out(o.view(x.shape[0], -1))
@@ -117,21 +133,15 @@ class BertLayer(nn.Module):
         self.norm2 = FusedAddLayerNorm(cfg.hidden_size, eps=cfg.layer_norm_eps)
         self.dropout = nn.Dropout(cfg.dropout)
 
-    def forward(self, x):
-        x = self.norm1(self.dropout(self.attn(x)), x)
-        return self.norm2(self.dropout(self.mlp(x)), x)
-
-    def packed(self, x, cu_seqlens, p, seed, offset):
-        """One block on a packed batch; its masks have offsets ``offset`` to
+    def forward(self, x, cu_seqlens=None, seed=None, offset=0):
+        """On a packed batch the block's masks have offsets ``offset`` to
         ``offset + 2``."""
-        from bluefog_amd.ops.transformer import layer_norm
-
-        def join(norm, y, x, offset):
-            return layer_norm(y, norm.weight, norm.bias, norm.eps, residual=x,
-                              dropout_p=p, seed=seed, offset=offset)
-
-        x = join(self.norm1, self.attn.packed(x, cu_seqlens, p, seed, offset), x, offset + 1)
-        return join(self.norm2, self.mlp(x), x, offset + 2)
+        if cu_seqlens is None:
+            x = self.norm1(self.dropout(self.attn(x)), x)
+            return self.norm2(self.dropout(self.mlp(x)), x)
+        p = _rate(self.dropout)
+        x = self.norm1(self.attn(x, cu_seqlens, seed, offset), x, (p, seed, offset + 1))
+        return self.norm2(self.mlp(x), x, (p, seed, offset + 2))
 
 
 class BertForMaskedLM(nn.Module):
@@ -187,12 +197,15 @@ class BertForMaskedLM(nn.Module):
                     f"{self.cfg.max_position_embeddings} positions"
                 )
             cu_seqlens = cu_seqlens.to(input_ids.device)
-        p = self.cfg.dropout if self.training else 0.0
         # one seed for a step; every mask of it has an offset of its own
-        seed = torch.randint(1 << 62, (1,), device=input_ids.device) if p else None
-        x = self.embeddings.packed(input_ids, cu_seqlens, p, seed)
+        drops = any(
+            m.training and (m.dropout_p if isinstance(m, BertSelfAttention) else isinstance(m, nn.Dropout) and m.p)
+            for m in self.modules()
+        )
+        seed = torch.randint(1 << 62, (1,), device=input_ids.device) if drops else None
+        x = self.embeddings(input_ids, cu_seqlens, seed)
         for i, layer in enumerate(self.layers):
-            x = layer.packed(x, cu_seqlens, p, seed, 1 + 3 * i)
+            x = layer(x, cu_seqlens, seed, 1 + 3 * i)
         return x
 
 

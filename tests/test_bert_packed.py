@@ -159,3 +159,76 @@ def test_bert_packed_tokens_in_front_of_the_first_sequence():
         got = model(ids, cu_seqlens=torch.tensor([13, 50], dtype=torch.int32, device="cuda"))[13:50]
         alone = model(ids[13:50], cu_seqlens=torch.tensor([0, 37], dtype=torch.int32))
     assert (got - alone).abs().max() < 1e-5 * alone.abs().max()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_bert_packed_modes_and_rates_of_its_modules(device):
+    """A module in evaluation, or with a probability of its own, drops what it
+    says, not what the model was made with."""
+    model = _tiny_bert(0.2).to(device)
+    lengths, ids, _, cu = _packed_batch(device)
+    used = slice(0, sum(lengths))
+
+    def run():
+        torch.manual_seed(7)
+        return model(ids, cu_seqlens=cu)[used]
+
+    quiet = model.eval()(ids, cu_seqlens=cu)[used]
+    model.train()
+    dropped = run()
+    for part in (model.embeddings, model.layers):
+        part.eval()
+    assert torch.equal(run(), quiet)
+    model.train()
+    for m in model.modules():
+        if isinstance(m, torch.nn.Dropout):
+            m.p = 0.0
+        if hasattr(m, "dropout_p"):
+            m.dropout_p = 0.0
+    assert torch.equal(run(), quiet)
+    model.layers[1].dropout.p = 0.5
+    half = run()
+    assert not torch.equal(half, quiet) and not torch.equal(half, dropped)
+    model.layers[1].dropout = torch.nn.Identity()
+    assert torch.equal(run(), quiet)
+    model.layers[1].dropout = torch.nn.Dropout1d(0.1)
+    with pytest.raises(TypeError, match="Dropout1d"):
+        run()
+
+
+def test_bert_packed_calls_its_modules():
+    """Hooks of every module run, but for those of nn.Dropout, and what a hook
+    returns takes part."""
+    model = _tiny_bert(0.2)
+    _, ids, _, cu = _packed_batch("cpu")
+    called = []
+    for name, m in model.named_modules():
+        m.register_forward_hook(lambda m, args, out, name=name: called.append(name))
+    model(ids, cu_seqlens=cu)
+    idle = {n for n, m in model.named_modules() if isinstance(m, (torch.nn.Dropout, torch.nn.ModuleList))}
+    # the position table's and the types' modules are called too
+    assert set(called) == {n for n, _ in model.named_modules()} - idle
+    model.eval()
+    before = model(ids, cu_seqlens=cu)
+    model.layers[0].norm1.register_forward_hook(lambda m, args, out: out * 2)
+    assert not torch.equal(model(ids, cu_seqlens=cu), before)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_bert_packed_without_the_fused_norm(device, monkeypatch):
+    """BLUEFOG_FUSED_LN=0 takes the norm operator out of the packed path; the
+    masks are the same. Both norms are 32-bit sums of 64 terms."""
+    from bluefog_amd.ops import transformer
+
+    model = _tiny_bert(0.2).to(device)
+    lengths, ids, _, cu = _packed_batch(device)
+    used = slice(0, sum(lengths))
+
+    def run():
+        torch.manual_seed(7)
+        return model(ids, cu_seqlens=cu)[used]
+
+    want = run()
+    monkeypatch.setenv("BLUEFOG_FUSED_LN", "0")
+    monkeypatch.setattr(transformer, "layer_norm", None)
+    assert (run() - want).abs().max() < 1e-5 * want.abs().max()
