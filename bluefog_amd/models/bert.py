@@ -114,7 +114,7 @@ class BertSelfAttention(nn.Module):
         p = self.dropout_p if self.training else 0.0
         q, k, v = self.qkv(x).view(x.shape[0], 3, self.nh, self.hd).unbind(1)
         o = packed_attention(q, k, v, cu_seqlens, dropout_p=p, seed=seed, offset=offset)
-        return self.out(o.view(x.shape[0], -1))
+        return self.out(o.flatten(1))
 
 
 class BertLayer(nn.Module):

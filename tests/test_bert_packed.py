@@ -232,3 +232,12 @@ def test_bert_packed_without_the_fused_norm(device, monkeypatch):
     monkeypatch.setenv("BLUEFOG_FUSED_LN", "0")
     monkeypatch.setattr(transformer, "layer_norm", None)
     assert (run() - want).abs().max() < 1e-5 * want.abs().max()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_bert_packed_empty_batch(device):
+    model = _tiny_bert(0.1).to(device)
+    out = model(torch.zeros(0, dtype=torch.int64, device=device), cu_seqlens=torch.zeros(1, dtype=torch.int32))
+    assert out.shape == (0, 97)
+    out.sum().backward()
+    assert all(not p.grad.any() for p in model.parameters() if p.grad is not None)
