@@ -1197,3 +1197,22 @@ def test_numbers_that_leave_32_bits_are_refused(device):
         wide = [t.double() for t in (q, k, v)]
         assert torch.isfinite(bf.packed_attention(*wide, cu, scale=1e-60)).all()
         assert not bf.layer_norm(x.double(), eps=1e-60).any()
+
+
+# ---------------------------------------------------------------------------
+# norms of more rows than a launch has workgroups for at once
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,width", [(16400 + 3, 96), (8200 + 3, 1001), (4200, 2051), (2100, 4096), (1100, 5000),
+                                        (1030, 8192), (600, 12289), (1030, 16385), (70, 40001), (9000, 5)])
+def test_norm_takes_row_after_row(dtype, rows, width):
+    """A workgroup has 4 rows at once up to a width of 1024 and 1 above; 8192 rows
+    are under way in the forward pass then (4096 in the backward pass), 2048 (1024)
+    up to 4096 columns, 1024 (512) up to 8192 and 512 (256) beyond, in the wide
+    kernels 64 for the sums over rows: every workgroup here takes more than one,
+    some one more than others."""
+    norm_agrees("cuda", dtype, (rows, width), seed=width)
+    norm_agrees("cuda", dtype, (rows, width), residual=dtype, weights=dtype, p=0.2, seed=width + 1)
