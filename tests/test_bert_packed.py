@@ -241,3 +241,59 @@ def test_bert_packed_empty_batch(device):
     assert out.shape == (0, 97)
     out.sum().backward()
     assert all(not p.grad.any() for p in model.parameters() if p.grad is not None)
+
+
+def _attentive_bert():
+    """Attention outweighs the residual: its weights are ten times as large, so
+    that scores have a size of 2 and its branch one of 2 beside a residual of 1."""
+    model = _tiny_bert().eval()
+    with torch.no_grad():
+        for layer in model.layers:
+            for part in (layer.attn.qkv, layer.attn.out):
+                part.weight *= 10
+    return model
+
+
+def _off(got, want):
+    return float((got.double().cpu() - want).norm() / want.norm())
+
+
+def _half_bound(dtype):
+    """The relative error of the logits: 8 roundings in each of two blocks and one
+    of the head, each of u = eps / 2 of its value at most, add up like their root;
+    norms, softmax and the larger weights pass on at most 4 times as much."""
+    return torch.finfo(dtype).eps / 2 * 17 ** 0.5 * 4
+
+
+@pytest.mark.parametrize("mistake", ["no attention", "causal"])
+def test_bert_packed_half_precision_bound_tells(mistake, monkeypatch):
+    """An attention that gives nothing, or that is causal, is far outside of it."""
+    from bluefog_amd.ops import transformer
+
+    model = _attentive_bert().double()
+    lengths, ids, _, cu = _packed_batch("cpu")
+    used, right = slice(0, sum(lengths)), transformer.packed_attention
+    with torch.no_grad():
+        want = model(ids, cu_seqlens=cu)[used]
+        monkeypatch.setattr(transformer, "packed_attention", lambda q, *a, **kw: (
+            torch.zeros_like(q) if mistake == "no attention" else right(q, *a, **kw, causal=True)))
+        off = _off(model(ids, cu_seqlens=cu)[used], want)
+    assert off > 4 * _half_bound(torch.bfloat16)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_bert_packed_half_precision_where_attention_counts(device, dtype):
+    model = _attentive_bert()
+    lengths, ids, _, cu = _packed_batch(device)
+    used = slice(0, sum(lengths))
+    with torch.no_grad():
+        want = copy.deepcopy(model).double()(ids.cpu(), cu_seqlens=cu)[used]
+        model = model.to(device)
+        with torch.autocast(device, dtype=dtype):
+            a = model(ids, cu_seqlens=cu)[used]
+        rounded = model.to(dtype)
+        b = rounded(ids, cu_seqlens=cu)[used]
+        # weights of the type are other weights: they have a result of their own
+        want_b = copy.deepcopy(rounded).cpu().double()(ids.cpu(), cu_seqlens=cu)[used]
+    assert _off(a, want) < _half_bound(dtype) and _off(b, want_b) < _half_bound(dtype)

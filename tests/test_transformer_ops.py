@@ -1200,6 +1200,76 @@ def test_numbers_that_leave_32_bits_are_refused(device):
 
 
 # ---------------------------------------------------------------------------
+# how exact half-precision gradients are
+# ---------------------------------------------------------------------------
+
+
+def times_the_last_rounding(got, exact, dtype):
+    """The error's size as a multiple of what rounding the exact result costs."""
+    own = exact.to(dtype).double() - exact
+    return float((got.detach().cpu().double() - exact).norm() / own.norm())
+
+
+def exact_gradients(q, k, v, dout, causal, rounded=None):
+    """out, dq, dk, dv in 64 bits for one sequence. ``rounded``: a mistake that
+    is planted, 'dS' rounded to the type in front of its products (f16: times a
+    power of two that keeps a row's largest near the type's), or 'delta' from
+    the rounded output."""
+    Q, K, V, G = (t.detach().cpu().double().transpose(0, 1) for t in (q, k, v, dout))
+    group, scale = Q.shape[0] // K.shape[0], Q.shape[2] ** -0.5
+    K, V = K.repeat_interleave(group, 0), V.repeat_interleave(group, 0)
+    S = Q @ K.transpose(1, 2) * scale
+    if causal:
+        S = S.masked_fill(~torch.ones(S.shape[1:], dtype=torch.bool).tril(), -math.inf)
+    P = torch.softmax(S, 2)
+    O = P @ V
+    delta = (G * (O.to(q.dtype).double() if rounded == "delta" else O)).sum(2, keepdim=True)
+    dS = P * (G @ V.transpose(1, 2) - delta)
+    if rounded == "dS":
+        power = 2.0 ** -torch.frexp(dS.abs().amax(2, keepdim=True).clamp_min(1e-30)).exponent
+        dS = (dS * power).to(q.dtype).double() / power
+    shared = [t.unflatten(0, (-1, group)).sum(1) for t in (dS.transpose(1, 2) @ Q * scale, P.transpose(1, 2) @ G)]
+    return {n: t.transpose(0, 1) for n, t in zip(("out", "dq", "dk", "dv"), (O, dS @ K * scale, *shared))}
+
+
+# Queries and keys of size 2: scores of 2 * 2 * sqrt(dim) / sqrt(dim) = 4 let softmax
+# pick keys that lie along the query. Those have a common part, and delta's error,
+# which goes into all dS of a row at once, moves dq by it.
+EXACT = [(1200, 4, 2, 64, False), (1200, 4, 2, 64, True), (900, 4, 1, 128, True), (900, 2, 2, 128, False), (500, 6, 2, 80, True)]
+# 1: nothing but the last rounding. A rounding more, of a value of the same relative
+# precision in every term of a sum with signs at random, adds as much again: sqrt(2).
+# dS carries what its rounding took, so dq and dk stay below that; P is rounded
+# once in front of out and dv, and nothing else is: below sqrt(3), two more.
+MOST_TIMES = {"dq": 1.3, "dk": 1.3, "out": 1.5, "dv": 1.5}
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("case", EXACT)
+def test_attention_is_as_exact_as_its_last_rounding(device, dtype, case):
+    n, heads, kv_heads, dim, causal = case
+    q, k, v, dout = attention_inputs((n,), heads, kv_heads, dim, dtype, device, seed=n, factor=2.0)
+    got = attention(q, k, v, dout, ends_of((n,), device), causal=causal)
+    exact = exact_gradients(q, k, v, dout, causal)
+    times = {name: times_the_last_rounding(got[name], exact[name], dtype) for name in exact}
+    assert all(times[name] < MOST_TIMES[name] for name in times), times
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("case", EXACT)
+def test_a_rounding_more_is_found(dtype, case):
+    """The bounds of the test above tell: dS rounded once, or delta from the
+    rounded output, leaves dq and dk outside."""
+    n, heads, kv_heads, dim, causal = case
+    q, k, v, dout = attention_inputs((n,), heads, kv_heads, dim, dtype, "cpu", seed=n, factor=2.0)
+    exact = exact_gradients(q, k, v, dout, causal)
+    for mistake in ("dS", "delta"):
+        off = exact_gradients(q, k, v, dout, causal, mistake)
+        times = {m: times_the_last_rounding(off[m].to(dtype), exact[m], dtype) for m in ("dq", "dk")}
+        assert all(times[m] > MOST_TIMES[m] for m in times), (mistake, times)
+
+
+# ---------------------------------------------------------------------------
 # norms of more rows than a launch has workgroups for at once
 # ---------------------------------------------------------------------------
 
