@@ -1286,3 +1286,38 @@ def test_norm_takes_row_after_row(dtype, rows, width):
     some one more than others."""
     norm_agrees("cuda", dtype, (rows, width), seed=width)
     norm_agrees("cuda", dtype, (rows, width), residual=dtype, weights=dtype, p=0.2, seed=width + 1)
+
+
+@pytest.mark.gpu
+def test_many_sequences_in_captured_graphs():
+    """The table of the tiles is made anew at every replay, from the bounds of
+    that replay; two graphs' tables are their own."""
+    g = torch.Generator().manual_seed(3)
+
+    def bounds(most):
+        ends = torch.randint(0, most + 1, (150,), generator=g).sort().values
+        ends[0] = 0
+        return ends.to(torch.int32).cuda()
+
+    static = [(*attention_inputs((n,), 4, 2, 64, torch.bfloat16, "cuda", seed=n), bounds(n)) for n in (900, 2000)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for s in static:
+            attention(*s, causal=True)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for s in static:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(attention(*s, causal=True))
+        graphs.append(graph)
+    for _ in range(4):
+        for s in static:
+            s[4].copy_(bounds(len(s[0])))
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for s, out in zip(static, outs):
+            for name, t in attention(*s, causal=True).items():
+                assert torch.equal(out[name], t)
