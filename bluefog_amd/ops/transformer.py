@@ -20,8 +20,9 @@ seed and offset, and the backward pass computes it again.
 
 GPU tensors (f32, f16, bf16) run gfx950 kernels and raise if the native
 extension is missing; CPU tensors (f64 too) run the torch code below. The
-results are differentiable once: ``create_graph=True`` raises on the GPU.
-Results do not depend on the order of atomics: there are none.
+results are differentiable once: ``create_graph=True`` and forward mode raise
+on the GPU, as do tensors without memory (fakes, freed storages). Results do
+not depend on the order of atomics: there are none.
 
 ``seed`` is an int, or one int64 on the device, which a captured graph reads
 at every replay; ``None`` draws one from torch's generator, so
@@ -125,7 +126,7 @@ def packed_attention(
         prob = torch.softmax(score, 2)
         if dropout_p:
             prob = _masked(prob, _attention_bits(heads, begin, n, key, offset, q.device), dropout_p)
-        if causal and not torch.isfinite(sv).all():
+        if causal and not _all_finite(sv):
             # a masked probability of 0 times such a value would be no number
             out = [torch.matmul(prob[:, i : i + 1, : i + 1], sv[:, : i + 1]) for i in range(n)]
             out = torch.cat(out, 1)
@@ -251,6 +252,13 @@ def _check(x: torch.Tensor, p: float, offset: int) -> None:
         raise ValueError(f"dropout probability has to be in [0, 1), got {p}")
     if not 0 <= offset <= _M32:
         raise ValueError(f"offset has to be in [0, 2^32), got {offset}")
+
+
+def _all_finite(x: torch.Tensor) -> bool:
+    try:
+        return bool(torch.isfinite(x).all())
+    except RuntimeError:  # inside torch.vmap, where no value can be asked for
+        return True
 
 
 def _philox(c0, c1, c2, c3, key: int) -> torch.Tensor:

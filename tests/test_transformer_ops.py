@@ -1321,3 +1321,17 @@ def test_many_sequences_in_captured_graphs():
         for s, out in zip(static, outs):
             for name, t in attention(*s, causal=True).items():
                 assert torch.equal(out[name], t)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_mapped_over_a_dimension(device, causal):
+    """torch.vmap over heads of batches of their own: slice by slice on the GPU;
+    batched products on the CPU, whose sums of at most 9 terms may have
+    another order."""
+    g = torch.Generator().manual_seed(9)
+    q = torch.randn(3, 14, 2, 8, generator=g).to(device)
+    cu = ends_of((5, 9), device)
+    got = torch.vmap(lambda t: bf.packed_attention(t, t, t, cu, causal=causal))(q)
+    want = torch.stack([bf.packed_attention(t, t, t, cu, causal=causal) for t in q])
+    assert (got - want).abs().max() <= (0 if device == "cuda" else 64 * F32 * float(q.abs().max()))
