@@ -46,6 +46,10 @@ void check(hipError_t e, const char* what) {
   TORCH_CHECK(e == hipSuccess, "bluefog_amd ", what, ": ", hipGetErrorString(e));
 }
 
+// Torch may leave a negation to whoever reads the memory (the imaginary part of a
+// conjugate): a copy then.
+Tensor plain(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+
 // A fake tensor, or one whose storage was freed, is a GPU tensor with nowhere to
 // read: a kernel would fault.
 void with_memory(const char* what, std::initializer_list<const Tensor*> ts) {
@@ -197,7 +201,7 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
     with_memory("packed_attention backward", {&q, &k, &v, &cu, &seed_tensor, &out, &lse, &rest, &table, &grads[0]});
     c10::DeviceGuard guard(q.device());
     const bool need_dkv = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
-    const Tensor dout = readable(grads[0]);
+    const Tensor dout = readable(plain(grads[0]));
     Tensor dq = at::empty(out.sizes(), out.options());
     Tensor dk = at::empty(k.sizes(), k.options(), at::MemoryFormat::Contiguous);
     Tensor dv = at::empty(v.sizes(), v.options(), at::MemoryFormat::Contiguous);
@@ -258,7 +262,7 @@ Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
                     " sequences, ", q.size(0), " tokens");
   with_memory("packed_attention", {&q, &k, &v, &cu, &st});
   no_tangents("packed_attention", {&q, &k, &v});
-  const Tensor rq = readable(q), rk = readable(k), rv = readable(v);
+  const Tensor rq = readable(plain(q)), rk = readable(plain(k)), rv = readable(plain(v));
   if (grad) return PackedAttention::apply(rq, rk, rv, cu, seed_tensor, scale, causal, p, seed, offset);
   return attn_forward(rq, rk, rv, cu, scale, causal, dropout_args(st, seed, offset, p), nullptr, nullptr, nullptr);
 }
@@ -374,7 +378,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
       return got;
     }
     const auto [rx, x_row] = as_rows(x);
-    const auto [rdy, dy_row] = as_rows(grads[0]);
+    const auto [rdy, dy_row] = as_rows(plain(grads[0]));
     a.x = rx.const_data_ptr(), a.x_row = x_row;
     a.dy = rdy.const_data_ptr(), a.dy_row = dy_row;
     Tensor hold;
@@ -403,7 +407,8 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, double eps,
                   const std::optional<Tensor>& residual, double p, const std::optional<Tensor>& seed_tensor,
                   int64_t seed, int64_t offset) {
-  const Tensor r = residual.value_or(Tensor()), st = seed_tensor.value_or(Tensor());
+  Tensor r = residual.value_or(Tensor());
+  const Tensor st = seed_tensor.value_or(Tensor());
   Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
   TORCH_CHECK_VALUE(x.is_cuda() && x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= 1 << 26,
                     "layer_norm needs a GPU tensor with a last dimension of 1 to 2^26");
@@ -428,13 +433,15 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const st
   with_memory("layer_norm", {&x, &r, &w, &b, &st});
   no_tangents("layer_norm", {&x, &r, &w, &b});
   const bool grad = any_grad({&x, &r, &w, &b});
-  if (w.defined()) w = w.contiguous();
-  if (b.defined()) b = b.contiguous();
+  const Tensor in = plain(x);
+  r = plain(r);
+  if (w.defined()) w = plain(w).contiguous();
+  if (b.defined()) b = plain(b).contiguous();
   if (grad) {
     const auto given = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
-    return LayerNorm::apply(x, given(r), given(w), given(b), given(st), eps, p, seed, offset);
+    return LayerNorm::apply(in, given(r), given(w), given(b), given(st), eps, p, seed, offset);
   }
-  return norm_forward(x, r, w, b, eps, dropout_args(st, seed, offset, p), nullptr, nullptr);
+  return norm_forward(in, r, w, b, eps, dropout_args(st, seed, offset, p), nullptr, nullptr);
 }
 
 // ---------------------------------------------------------------------------
@@ -469,7 +476,7 @@ struct CounterDropout : torch::autograd::Function<CounterDropout> {
     if (!grads[0].defined()) return got;
     const Tensor seed_tensor = ctx->get_saved_variables()[0];
     with_memory("counter_dropout backward", {&seed_tensor});
-    got[0] = masked(grads[0], dropout_args(seed_tensor, ctx->saved_data["seed"].toInt(),
+    got[0] = masked(plain(grads[0]), dropout_args(seed_tensor, ctx->saved_data["seed"].toInt(),
                                            ctx->saved_data["offset"].toInt(), ctx->saved_data["p"].toDouble()));
     return got;
   }
@@ -484,8 +491,8 @@ Tensor counter_dropout(const Tensor& x, double p, const std::optional<Tensor>& s
   with_memory("counter_dropout", {&x, &st});
   no_tangents("counter_dropout", {&x});
   const bool grad = any_grad({&x});
-  if (grad) return CounterDropout::apply(x, seed_tensor, p, seed, offset);
-  return masked(x, dropout_args(st, seed, offset, p));
+  if (grad) return CounterDropout::apply(plain(x), seed_tensor, p, seed, offset);
+  return masked(plain(x), dropout_args(st, seed, offset, p));
 }
 
 // the operator `name` as torch's dispatcher calls it, with F's arguments

@@ -1335,3 +1335,40 @@ def test_attention_mapped_over_a_dimension(device, causal):
     got = torch.vmap(lambda t: bf.packed_attention(t, t, t, cu, causal=causal))(q)
     want = torch.stack([bf.packed_attention(t, t, t, cu, causal=causal) for t in q])
     assert (got - want).abs().max() <= (0 if device == "cuda" else 64 * F32 * float(q.abs().max()))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("which", range(5))
+def test_negated_views(device, which):
+    """The imaginary part of a conjugate is a view whose values are the memory's
+    times -1: as an argument and as an upstream gradient. Its last dimension
+    counts as dense where it has one value."""
+    def negated(t):
+        view = torch.imag(torch.complex(torch.zeros_like(t), -t).conj())
+        assert view.is_neg() and torch.equal(view, t)
+        return view
+
+    calls = calls_of_all(device)
+    q, k, v, _ = (t.detach() for t in attention_inputs((5, 9), 4, 2, 1, torch.float32, device))
+    cu = ends_of((5, 9), device)
+    calls.append((lambda q, k, v: bf.packed_attention(q, k, v, cu), (q, k, v)))
+    x, r, w, b, _ = (t.detach() for t in norm_inputs((6, 1), torch.float32, device, residual=torch.float32))
+    calls.append((lambda x, r, w, b: bf.layer_norm(x, w, b, residual=r), (x, r, w, b)))
+    f, args = calls[which]
+    leaves = [t.clone().requires_grad_() for t in args]
+    want = f(*leaves)
+    up = torch.randn(want.shape, generator=torch.Generator().manual_seed(1)).to(device)
+    want_grads = torch.autograd.grad(want, leaves, up)
+    views = [negated(t).detach().requires_grad_() for t in args]
+    got = f(*views)
+    assert torch.equal(got, want)
+    for g, w in zip(torch.autograd.grad(got, views, negated(up)), want_grads):
+        assert torch.equal(g, w)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_in_inference_mode(device):
+    for f, args in calls_of_all(device):
+        with torch.inference_mode():
+            got = f(*args)
+        assert torch.equal(got, f(*args))
