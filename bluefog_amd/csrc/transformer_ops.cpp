@@ -50,6 +50,10 @@ void check(hipError_t e, const char* what) {
 // conjugate): a copy then.
 Tensor plain(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
 
+// Saved tensors as the kernels read them: hooks may bring back the same values in
+// another layout (torch.autograd.graph.saved_tensors_hooks).
+Tensor dense(const Tensor& t) { return !t.defined() || t.is_contiguous() ? t : t.contiguous(); }
+
 // A fake tensor, or one whose storage was freed, is a GPU tensor with nowhere to
 // read: a kernel would fault.
 void with_memory(const char* what, std::initializer_list<const Tensor*> ts) {
@@ -197,8 +201,9 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
     variable_list none(10);
     if (!grads[0].defined()) return none;
     const variable_list s = ctx->get_saved_variables();
-    const Tensor &q = s[0], &k = s[1], &v = s[2], &cu = s[3], &seed_tensor = s[4], &out = s[5], &lse = s[6], &rest = s[7], &table = s[8];
-    with_memory("packed_attention backward", {&q, &k, &v, &cu, &seed_tensor, &out, &lse, &rest, &table, &grads[0]});
+    with_memory("packed_attention backward", {&s[0], &s[1], &s[2], &s[3], &s[4], &s[5], &s[6], &s[7], &s[8], &grads[0]});
+    const Tensor q = readable(s[0]), k = readable(s[1]), v = readable(s[2]), cu = dense(s[3]), &seed_tensor = s[4];
+    const Tensor out = dense(s[5]), lse = dense(s[6]), rest = dense(s[7]), table = dense(s[8]);
     c10::DeviceGuard guard(q.device());
     const bool need_dkv = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
     const Tensor dout = readable(plain(grads[0]));
@@ -353,8 +358,9 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     variable_list got(9);
     if (!grads[0].defined()) return got;
     const variable_list s = ctx->get_saved_variables();
-    const Tensor &x = s[0], &r = s[1], &weight = s[2], &bias = s[3], &seed_tensor = s[4];
-    with_memory("layer_norm backward", {&x, &r, &weight, &bias, &seed_tensor, &s[5], &s[6], &grads[0]});
+    with_memory("layer_norm backward", {&s[0], &s[1], &s[2], &s[3], &s[4], &s[5], &s[6], &grads[0]});
+    const Tensor &x = s[0], &r = s[1], &seed_tensor = s[4];
+    const Tensor weight = dense(s[2]), bias = dense(s[3]), mean = dense(s[5]), rstd = dense(s[6]);
     c10::DeviceGuard guard(x.device());
     BfNormArgs a = norm_args(x, weight, bias, ctx->saved_data["eps"].toDouble(),
                              dropout_args(seed_tensor, ctx->saved_data["seed"].toInt(),
@@ -387,8 +393,8 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
       hold = rr;
       a.r = rr.const_data_ptr(), a.r_row = r_row;
     }
-    a.mean = s[5].data_ptr<float>();
-    a.rstd = s[6].data_ptr<float>();
+    a.mean = mean.data_ptr<float>();
+    a.rstd = rstd.data_ptr<float>();
     a.dx = got[0].defined() ? got[0].data_ptr() : nullptr;
     a.dr = got[1].defined() && !got[1].is_same(got[0]) ? got[1].data_ptr() : nullptr;
     a.dweight = got[2].defined() ? got[2].data_ptr() : nullptr;

@@ -1372,3 +1372,35 @@ def test_in_inference_mode(device):
         with torch.inference_mode():
             got = f(*args)
         assert torch.equal(got, f(*args))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [16, 7])
+def test_saved_tensors_in_another_layout(dim):
+    """Hooks that keep what the forward pass saves, and bring it back with its
+    values but other strides, give the same gradients."""
+    device = "cuda"
+    q, k, v, dout = attention_inputs((70,) + (3,) * 80, 4, 2, dim, torch.bfloat16, device)
+    cu = ends_of((70,) + (3,) * 80, device)
+    x, r, w, b, dy = norm_inputs((6, 24), torch.bfloat16, device, residual=torch.bfloat16)
+    kw = dict(dropout_p=0.2, seed=torch.tensor([3], device=device))
+
+    def results():
+        return [bf.packed_attention(q, k, v, cu, **kw), bf.layer_norm(x, w, b, residual=r, **kw)]
+
+    def grads(outs):
+        return [*torch.autograd.grad(outs[0], (q, k, v), dout), *torch.autograd.grad(outs[1], (x, r, w, b), dy)]
+
+    want = grads(results())
+    apart = []
+
+    def unpack(t):
+        t = torch.stack([t, t + 1], -1)[..., 0]
+        apart.append(t.dim() and t.stride(-1) == 2)
+        return t
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), unpack):
+        outs = results()
+    for g, t in zip(grads(outs), want):
+        assert torch.equal(g, t)
+    assert any(apart)
