@@ -626,7 +626,7 @@ hipError_t dispatch(const BfNormArgs& a, int x_dtype, int r_dtype, hipStream_t s
 template <typename T>
 hipError_t drop(void* y, const void* x, long n, const BfDropout& d, hipStream_t stream) {
   const long blocks = (n + 256 * kVec - 1) / (256 * kVec);
-  if (blocks > 0xFFFFFF) return hipErrorInvalidValue;  // a launch has less than 2^32 threads
+  if (n > bf_dropout_most()) return hipErrorInvalidValue;
   hipLaunchKernelGGL(dropout_k<T>, dim3(blocks), dim3(256), 0, stream, static_cast<T*>(y), static_cast<const T*>(x), n,
                      d);
   return hipGetLastError();
@@ -645,6 +645,8 @@ hipError_t bf_norm_bwd(const BfNormArgs* a, int x_dtype, int r_dtype, hipStream_
 }
 
 long bf_norm_partial_floats(long rows, int width) { return 2L * width * slots_of(rows, width); }
+
+long bf_dropout_most() { return 0xFFFFFFL * 256 * kVec; }  // a launch has less than 2^32 threads
 
 hipError_t bf_dropout(void* y, const void* x, long n, int dtype, const BfDropout* d, hipStream_t stream) {
   switch (dtype) {

@@ -66,6 +66,7 @@ hipError_t bf_norm_fwd(const BfNormArgs* a, int x_dtype, int r_dtype,
 hipError_t bf_norm_bwd(const BfNormArgs* a, int x_dtype, int r_dtype,
                        hipStream_t stream);
 long bf_norm_partial_floats(long rows, int width);
+long bf_dropout_most();  // values of a call
 hipError_t bf_dropout(void* y, const void* x, long n, int dtype,
                       const BfDropout* d, hipStream_t stream);
 }

@@ -494,6 +494,7 @@ Tensor counter_dropout(const Tensor& x, double p, const std::optional<Tensor>& s
   TORCH_CHECK_VALUE(x.is_cuda(), "counter_dropout needs a GPU tensor");
   check_dropout(x, st, offset, p);
   code_of(x);
+  TORCH_CHECK_VALUE(x.numel() <= bf_dropout_most(), "counter_dropout takes at most ", bf_dropout_most(), " values, got ", x.numel());
   with_memory("counter_dropout", {&x, &st});
   no_tangents("counter_dropout", {&x});
   const bool grad = any_grad({&x});

@@ -204,7 +204,8 @@ def layer_norm(
 def counter_dropout(x: torch.Tensor, p: float, seed: Seed = None, offset: int = 0) -> torch.Tensor:
     """x with a share p of its elements set to 0 and the others scaled by
     1 / (1 - p). The mask depends on seed, offset and the place of an element
-    in row-major order, not on x's strides."""
+    in row-major order, not on x's strides. A GPU call takes fewer than 2**35
+    elements."""
     if x.is_cuda and hip_ext._require_ext("counter_dropout"):
         seed, value = _seed(seed, x, p)
         return hip_ext._C.counter_dropout(x, p, seed, value, offset)

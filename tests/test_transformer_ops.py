@@ -1404,3 +1404,16 @@ def test_saved_tensors_in_another_layout(dim):
     for g, t in zip(grads(outs), want):
         assert torch.equal(g, t)
     assert any(apart)
+
+
+def test_dropout_refuses_more_than_a_launch_holds():
+    """With what it is, before anything runs. Fake tensors: nothing is launched."""
+    from torch._subclasses import FakeTensorMode
+
+    if not hip_ext.has_extension():
+        pytest.skip("the native extension is not built")
+    with FakeTensorMode():
+        x = torch.empty((1 << 35) - 2048, dtype=torch.float16, device="cuda")
+        refused(NotImplementedError, "memory", bf.counter_dropout, x, 0.1, 1)
+        x = torch.empty((1 << 35) - 2047, dtype=torch.float16, device="cuda")
+        refused(ValueError, "at most", bf.counter_dropout, x, 0.1, 1)
