@@ -297,3 +297,39 @@ def test_bert_packed_half_precision_where_attention_counts(device, dtype):
         # weights of the type are other weights: they have a result of their own
         want_b = copy.deepcopy(rounded).cpu().double()(ids.cpu(), cu_seqlens=cu)[used]
     assert _off(a, want) < _half_bound(dtype) and _off(b, want_b) < _half_bound(dtype)
+
+
+@pytest.mark.gpu
+def test_bert_packed_captured_dropout():
+    """A captured step draws new masks at every replay, the same ones in its
+    forward and backward pass: replayed from torch's seed it repeats the eager
+    step."""
+    model = _tiny_bert(0.3).cuda()
+    _, ids, labels, cu = _packed_batch("cuda")
+    cu, params = cu.cuda(), list(model.parameters())
+
+    def step():
+        loss = model(ids, labels=labels, cu_seqlens=cu)
+        return [loss.detach(), *torch.autograd.grad(loss, params)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    losses = []
+    for n in range(4):
+        torch.manual_seed(20 + n)
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = [t.clone() for t in got]
+        losses.append(replayed[0].item())
+        torch.manual_seed(20 + n)
+        # the library's sums over the embeddings' rows have no fixed order
+        for a, b in zip(replayed, step()):
+            assert (a - b).abs().max() <= 1e-5 * b.abs().max() + 1e-8
+    assert len(set(losses)) == 4

@@ -1417,3 +1417,12 @@ def test_dropout_refuses_more_than_a_launch_holds():
         refused(NotImplementedError, "memory", bf.counter_dropout, x, 0.1, 1)
         x = torch.empty((1 << 35) - 2047, dtype=torch.float16, device="cuda")
         refused(ValueError, "at most", bf.counter_dropout, x, 0.1, 1)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_many_sequences_with_dropout(device, dtype, causal):
+    """Their masks go by the packed row, whichever way its sequence is found."""
+    lengths = [n % 7 for n in range(100)] + [135, 20]
+    attention_agrees(device, dtype, lengths, 4, 2, 32, causal=causal, p=0.2, spare=3)
